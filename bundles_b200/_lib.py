@@ -7,7 +7,7 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libb200nodes.so")
 
-vp, i32, f32, sz = C.c_void_p, C.c_int, C.c_float, C.c_size_t
+vp, i32, i64, f32, sz = C.c_void_p, C.c_int, C.c_longlong, C.c_float, C.c_size_t
 
 
 class MoeLists(C.Structure):
@@ -60,6 +60,11 @@ PROTOTYPES = {
     "b200_attn_verify_splits": (i32, [i32]),
     "b200_attn_verify_workspace_bytes": (sz, [i32, i32]),
     "b200_attn_verify": (i32, [vp, vp, vp, vp, vp, vp, i32, vp, i32, vp, i32, f32, i32, vp, vp, sz, vp, vp]),
+    "b200_page_plan": (i32, [vp, vp, i32, vp, i32, i32, vp, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp]),
+    "b200_kv_append": (i32, [vp, vp, i64, i64, i32, i32, i32, i32, vp, vp, i32, vp, vp, vp]),
+    "b200_attn_extend_workspace_bytes": (sz, [i32, i32, i32, i32]),
+    "b200_attn_extend": (i32, [vp, i64, vp, i64, vp, vp, i32, vp, i32, vp, vp, i32, i32, i32, i32, i32, i32, f32, vp, vp, sz,
+                               vp, vp]),
     "b200_dense_fp8_workspace_bytes": (sz, [i32, i32]),
     "b200_dense_fp8": (i32, [vp, i32, i32, vp, vp, i32, vp, vp, sz, vp, vp]),
     "b200_add_rmsnorm": (i32, [vp, vp, vp, f32, i32, i32, vp, vp]),

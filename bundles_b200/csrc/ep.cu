@@ -150,7 +150,7 @@ extern "C" int b200_set_wait_budget_ns(unsigned long long ns) {
   if (ns == 0) ns = WAIT_BUDGET_DEFAULT_NS;
   int (*setters[])(unsigned long long) = {set_wait_budget_router, set_wait_budget_moe,        set_wait_budget_moe_fp8,
                                           set_wait_budget_attn,   set_wait_budget_attn_verify, set_wait_budget_gdn,
-                                          set_wait_budget_ep};
+                                          set_wait_budget_ep,     set_wait_budget_attn_extend};
   for (auto f : setters) {
     const int rc = f(ns);
     if (rc != 0) return fail(rc, "b200_set_wait_budget_ns: %s", cudaGetErrorString(static_cast<cudaError_t>(rc)));

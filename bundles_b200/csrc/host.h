@@ -77,6 +77,7 @@ int set_wait_budget_moe(unsigned long long ns);
 int set_wait_budget_moe_fp8(unsigned long long ns);
 int set_wait_budget_attn(unsigned long long ns);
 int set_wait_budget_attn_verify(unsigned long long ns);
+int set_wait_budget_attn_extend(unsigned long long ns);
 int set_wait_budget_gdn(unsigned long long ns);
 int set_wait_budget_ep(unsigned long long ns);
 

@@ -1,0 +1,245 @@
+// The paged KV cache around the attention: block tables, positions and slot maps from request lengths
+// (page_plan_kernel), and the writer of a ragged batch of new tokens' K and V into the pages (kv_append).
+// No counterpart in the reference: its engine builds both on the host and hands the kernels a per-token table
+// (qk_attn_verify.cu:398-423).
+#include "common.cuh"
+#include "host.h"
+
+namespace b200 {
+
+constexpr int PG_TOKENS = 128;     // tokens of a page
+constexpr int PP_THREADS = 1024;
+constexpr int PP_MAX_BATCH = 8192;
+
+struct PlanArgs {
+  const int32_t* ctx;
+  const int32_t* fresh;     // new tokens per request
+  int B;
+  int32_t* table;           // [B, pt_stride]
+  int pt_stride, num_pages;
+  const int32_t* free_pages;
+  int free_cap;
+  const int32_t* n_free;
+  int T;
+  int32_t* cu;
+  int32_t* seqlens;
+  int64_t* positions;
+  int64_t* slots;
+  int32_t* n_left;
+  int32_t* status;
+};
+
+__device__ __forceinline__ void flag(int32_t* status, int code) {
+  if (status) atomicCAS(status, 0, code);
+}
+
+// Exclusive prefix sum over the CTA of one value per thread; `total` is the sum.  `tmp`: 33 words of shared memory.
+__device__ __forceinline__ long long block_scan(long long v, long long* tmp, long long& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  long long inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(FULL_MASK, inc, o);
+    if (lane >= o) inc += u;
+  }
+  if (lane == 31) tmp[warp] = inc;
+  __syncthreads();
+  if (warp == 0) {
+    long long w = lane < nw ? tmp[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(FULL_MASK, w, o);
+      if (lane >= o) w += u;
+    }
+    if (lane < nw) tmp[lane] = w;
+  }
+  __syncthreads();
+  total = tmp[nw - 1];
+  const long long before = (warp ? tmp[warp - 1] : 0) + inc - v;
+  __syncthreads();
+  return before;
+}
+
+// Last index b in [0, n) with a[b] <= x (a ascending, a[0] <= x).
+__device__ __forceinline__ int last_not_above(const int* a, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a[mid] <= x)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+// Every CTA forms the two prefix sums over the batch (first row and first new page of every request) in its own shared
+// memory and then fills its share of the token rows and of the new table entries: the CTAs exchange nothing, so one
+// launch does it all.  An entry that a token reads is either an old one, which nobody writes, or taken from the free
+// list directly, which nobody writes either.
+__global__ void __launch_bounds__(PP_THREADS) page_plan_kernel(const PlanArgs p) {
+  extern __shared__ int pp_smem[];
+  __shared__ long long tmp[33];
+  int* s_cu = pp_smem;                   // [B + 1] first row of a request
+  int* s_pg = pp_smem + p.B + 1;         // [B + 1] first new page of a request, counted over the batch
+  int* s_ctx = pp_smem + 2 * (p.B + 1);  // [B] tokens already cached
+  pdl_wait();
+  pdl_launch();
+  const int tid = threadIdx.x;
+  const bool first = blockIdx.x == 0;
+  const int per = (p.B + PP_THREADS - 1) / PP_THREADS, b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
+  const long long cap = static_cast<long long>(p.pt_stride) * PG_TOKENS;
+  long long sum = 0, total;
+  for (int b = b0; b < b1; ++b) {
+    const int n = p.fresh[b], c = p.ctx[b];
+    if (first && (n < 0 || c < 0)) flag(p.status, B200_ST_BAD_LEN);
+    if (first && c > cap) flag(p.status, B200_ST_NO_PAGE);
+    s_ctx[b] = static_cast<int>(min(static_cast<long long>(max(c, 0)), min(cap, 0x3fffffffll)));
+    sum += max(n, 0);
+  }
+  long long at = block_scan(sum, tmp, total);
+  if (first && tid == 0 && total > p.T) flag(p.status, B200_ST_BAD_LEN);
+  for (int b = b0; b < b1; ++b) {
+    s_cu[b] = static_cast<int>(min(at, static_cast<long long>(p.T)));
+    at += max(p.fresh[b], 0);
+  }
+  if (tid == 0) s_cu[p.B] = static_cast<int>(min(total, static_cast<long long>(p.T)));
+  __syncthreads();
+  sum = 0;
+  auto pages = [&](int b) -> int {   // new pages of request b inside the table
+    const int have = (s_ctx[b] + PG_TOKENS - 1) / PG_TOKENS;
+    const int need = (s_ctx[b] + (s_cu[b + 1] - s_cu[b]) + PG_TOKENS - 1) / PG_TOKENS;
+    return max(0, min(need, p.pt_stride) - have);
+  };
+  for (int b = b0; b < b1; ++b) sum += pages(b);
+  at = block_scan(sum, tmp, total);
+  for (int b = b0; b < b1; ++b) {
+    s_pg[b] = static_cast<int>(at);
+    at += pages(b);
+  }
+  if (tid == 0) s_pg[p.B] = static_cast<int>(total);
+  __syncthreads();
+  const int n_new = s_pg[p.B], n_tok = s_cu[p.B];
+  const int n_free = p.free_pages ? max(0, min(*p.n_free, p.free_cap)) : 0;
+  if (first) {
+    for (int b = tid; b <= p.B; b += PP_THREADS) {
+      p.cu[b] = s_cu[b];
+      if (b < p.B) p.seqlens[b] = s_ctx[b] + (s_cu[b + 1] - s_cu[b]);
+    }
+    if (tid == 0 && p.n_left) *p.n_left = max(0, n_free - n_new);
+  }
+  const int g0 = blockIdx.x * PP_THREADS + tid, gn = gridDim.x * PP_THREADS;
+  // the k-th new page of the batch comes off the end of the free list
+  auto taken = [&](int k) -> int {
+    if (k >= n_free) return -1;
+    const int id = p.free_pages[n_free - 1 - k];
+    return id >= 0 && id < p.num_pages ? id : -2;
+  };
+  if (p.free_pages)
+    for (int k = g0; k < n_new; k += gn) {
+      const int b = last_not_above(s_pg, p.B + 1, k);
+      const int id = taken(k);
+      if (id < 0) flag(p.status, id == -1 ? B200_ST_NO_PAGE : B200_ST_BAD_PAGE);
+      p.table[static_cast<size_t>(b) * p.pt_stride + (s_ctx[b] + PG_TOKENS - 1) / PG_TOKENS + (k - s_pg[b])] = max(id, -1);
+    }
+  for (int t = g0; t < p.T; t += gn) {
+    long long pos = 0, slot = -1;
+    if (t < n_tok) {
+      const int b = last_not_above(s_cu, p.B + 1, t);
+      pos = static_cast<long long>(s_ctx[b]) + (t - s_cu[b]);
+      const int j = static_cast<int>(pos / PG_TOKENS), have = (s_ctx[b] + PG_TOKENS - 1) / PG_TOKENS;
+      int id;
+      if (j >= p.pt_stride) {
+        id = -1;
+      } else if (j < have || !p.free_pages) {
+        id = p.table[static_cast<size_t>(b) * p.pt_stride + j];
+        if (id < 0 || id >= p.num_pages) id = -2;
+      } else {
+        id = taken(s_pg[b] + j - have);
+      }
+      if (id >= 0)
+        slot = static_cast<long long>(id) * PG_TOKENS + pos % PG_TOKENS;
+      else
+        flag(p.status, id == -1 ? B200_ST_NO_PAGE : B200_ST_BAD_PAGE);
+    }
+    p.positions[t] = pos;
+    p.slots[t] = slot;
+  }
+}
+
+// One CTA per (token, kv head).
+template <typename E>
+__global__ void __launch_bounds__(256) kv_append_rows_kernel(const E* __restrict__ k, const E* __restrict__ v,
+                                                             long long k_stride, long long v_stride, int hkv, int dim,
+                                                             E* __restrict__ kc, E* __restrict__ vc, int num_pages,
+                                                             const int64_t* __restrict__ slots, int32_t* status) {
+  pdl_wait();
+  pdl_launch();
+  const int t = blockIdx.x / hkv, h = blockIdx.x % hkv, d = threadIdx.x;
+  const long long slot = slots[t];
+  if (slot < 0) return;
+  const long long page = slot / PG_TOKENS;
+  const int o = static_cast<int>(slot % PG_TOKENS);
+  if (page >= num_pages) {
+    if (d == 0) flag(status, B200_ST_BAD_PAGE);
+    return;
+  }
+  const size_t ph = static_cast<size_t>(page) * hkv + h;
+  kc[(ph * PG_TOKENS + o) * dim + d] = k[t * k_stride + h * dim + d];
+  vc[(ph * dim + d) * PG_TOKENS + o] = v[t * v_stride + h * dim + d];
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int b200_page_plan(const int32_t* ctx_lens, const int32_t* new_lens, int B, int32_t* page_table, int pt_stride,
+                              int num_pages, const int32_t* free_pages, int free_cap, const int32_t* n_free, int T,
+                              int32_t* cu_seqlens, int32_t* seqlens, int64_t* positions, int64_t* slots, int32_t* n_left,
+                              int32_t* status, void* stream) {
+  if (!ctx_lens || !new_lens || !page_table || !cu_seqlens || !seqlens || !positions || !slots)
+    return fail(B200_E_ARG, "b200_page_plan: null pointer");
+  if (free_pages && (!n_free || !n_left)) return fail(B200_E_ARG, "b200_page_plan: a free list needs n_free and n_left");
+  if (B <= 0 || B > PP_MAX_BATCH || T <= 0 || pt_stride <= 0 || num_pages <= 0 || (free_pages && free_cap <= 0))
+    return fail(B200_E_ARG, "b200_page_plan: need 1 <= B <= %d, T, pt_stride, num_pages and free_cap >= 1 (B=%d T=%d)",
+                PP_MAX_BATCH, B, T);
+  if (pt_stride > (1 << 23) || T > (1 << 29)) return fail(B200_E_ARG, "b200_page_plan: pt_stride <= 2^23 and T <= 2^29");
+  static DeviceOnce once;
+  once.run([] {
+    cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (3 * PP_MAX_BATCH + 2) * 4);
+  });
+  const PlanArgs a{ctx_lens, new_lens, B,  page_table, pt_stride, num_pages, free_pages, free_cap,
+                   n_free,   T,        cu_seqlens, seqlens, positions, slots, n_left, status};
+  int grid = (T + PP_THREADS - 1) / PP_THREADS;
+  if (grid > sm_count()) grid = sm_count();
+  launch_k(page_plan_kernel, dim3(grid), dim3(PP_THREADS), (3 * static_cast<size_t>(B) + 2) * 4,
+           static_cast<cudaStream_t>(stream), a);
+  return launch_status("b200_page_plan");
+}
+
+extern "C" int b200_kv_append(const void* k, const void* v, long long k_stride, long long v_stride, int T, int Hkv, int D,
+                              int cache_bf16, void* kcache, void* vcache, int num_pages, const int64_t* slots,
+                              int32_t* status, void* stream) {
+  if (!k || !v || !kcache || !vcache || !slots) return fail(B200_E_ARG, "b200_kv_append: null pointer");
+  if (T < 0 || Hkv <= 0 || Hkv > 128 || (D != 128 && D != 256) || num_pages <= 0)
+    return fail(B200_E_ARG, "b200_kv_append: need T >= 0, 1 <= Hkv <= 128, D 128 or 256 and num_pages >= 1 (Hkv=%d D=%d)", Hkv,
+                D);
+  const long long es = cache_bf16 ? 2 : 1;
+  if (k_stride < static_cast<long long>(Hkv) * D || v_stride < static_cast<long long>(Hkv) * D)
+    return fail(B200_E_ARG, "b200_kv_append: a token stride is shorter than a token's row");
+  if (((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(kcache) |
+        reinterpret_cast<uintptr_t>(vcache) | static_cast<uintptr_t>(k_stride * es) | static_cast<uintptr_t>(v_stride * es)) & 15))
+    return fail(B200_E_ALIGN, "b200_kv_append: tensors and token strides must be 16-byte aligned");
+  if (T == 0) return 0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (static_cast<long long>(T) * Hkv > 0x7fffffffll) return fail(B200_E_ARG, "b200_kv_append: T * Hkv must stay below 2^31");
+  if (cache_bf16)
+    launch_k(kv_append_rows_kernel<uint16_t>, dim3(T * Hkv), dim3(D), 0, st, static_cast<const uint16_t*>(k),
+             static_cast<const uint16_t*>(v), k_stride, v_stride, Hkv, D, static_cast<uint16_t*>(kcache),
+             static_cast<uint16_t*>(vcache), num_pages, slots, status);
+  else
+    launch_k(kv_append_rows_kernel<uint8_t>, dim3(T * Hkv), dim3(D), 0, st, static_cast<const uint8_t*>(k),
+             static_cast<const uint8_t*>(v), k_stride, v_stride, Hkv, D, static_cast<uint8_t*>(kcache),
+             static_cast<uint8_t*>(vcache), num_pages, slots, status);
+  return launch_status("b200_kv_append");
+}

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -17,7 +18,7 @@ from ._lib import B200Error, MoeLists, MoeWeights, check
 
 __all__ = ["router", "RoutingLists", "build_lists", "MoeW8A8Weights", "moe_w8a8", "moe_w8a8_ep", "ep_push", "ep_put",
            "ep_barrier", "moe_fp8", "moe_fp8_ep", "moe_combine", "moe_combine_norm", "attn_front", "attn_verify",
-           "dense_fp8", "dense_fp8_split", "dense_fp8_add_rmsnorm", "add_rmsnorm", "lmhead_argmax", "argmax_merge", "gdn_verify",
+           "PagePlan", "page_plan", "kv_append", "attn_extend", "dense_fp8", "dense_fp8_split", "dense_fp8_add_rmsnorm", "add_rmsnorm", "lmhead_argmax", "argmax_merge", "gdn_verify",
            "gdn_verify_replay", "gdn_ring_fold", "set_wait_budget_ns", "selftest_wait_expiry", "new_status",
            "read_status", "B200Error"]
 
@@ -400,6 +401,174 @@ def attn_verify(q, gate, k_new, v_new, kcache, vcache, page_table, seqlens, scal
                                       _p(page_table), page_table.shape[1], _p(seqlens), B, float(scale), int(splits),
                                       _p(out), _p(ws), ws.numel(), _p(status), _stream()), "b200_attn_verify")
     return out
+
+
+class PagePlan(NamedTuple):
+    """What `page_plan` makes of a step's request lengths; all on the device."""
+    cu_seqlens: torch.Tensor    # int32 [B + 1]: first row of every request
+    seqlens: torch.Tensor       # int32 [B]: tokens of every request, the new ones included
+    positions: torch.Tensor     # int64 [max_tokens]: a row's place in its request (0 behind the last request)
+    slots: torch.Tensor         # int64 [max_tokens]: its place in the pool, page * 128 + place in the page (-1: none)
+    n_left: torch.Tensor        # int32 [1]: pages left on the free list
+
+
+def _launch(what, fn, device, *args):
+    """Calls `fn` on `device`'s current stream, whichever device is current."""
+    if device.index == torch.cuda.current_device():
+        check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+
+
+def _together(what, device, *tensors):
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise B200Error(f"{what}: tensors on {device} and {t.device}")
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _need_status(what, status, device):
+    if status is not None:
+        _need(status, torch.int32, "status")
+        _together(what, device, status)
+
+
+def _token_rows(t, dtype, name, heads=None, dim=None):
+    """[T, heads, dim] rows whose heads lie side by side; returns the token stride in elements."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dtype and t.dim() == 3):
+        raise B200Error(f"{name} must be a CUDA tensor [T, heads, dim] of {dtype}")
+    T, h, d = t.shape
+    if (heads is not None and h != heads) or (dim is not None and d != dim):
+        raise B200Error(f"{name} must be [T, {heads}, {dim}], got {tuple(t.shape)}")
+    st, sh, sd = t.stride()
+    if sd != 1 or (h > 1 and sh != d):
+        raise B200Error(f"{name}: a token's heads must be contiguous (strides {t.stride()})")
+    return st if T > 1 else h * d
+
+
+def _need_pages(kcache, vcache):
+    """The caches' (dtype, pages, kv heads, dim): K [P, Hkv, 128, D], V [P, Hkv, D, 128] in uint8 (e4m3 codes) or bf16."""
+    dt = kcache.dtype if isinstance(kcache, torch.Tensor) else None
+    if dt not in (torch.uint8, torch.bfloat16):
+        raise B200Error("kcache must hold e4m3 codes (uint8) or bf16")
+    _need(kcache, dt, "kcache", 4)
+    _need(vcache, dt, "vcache", 4)
+    P, hkv, page, D = kcache.shape
+    if page != 128 or tuple(vcache.shape) != (P, hkv, D, 128):
+        raise B200Error("the caches must be K [pages, kv heads, 128, dim] and V [pages, kv heads, dim, 128], got "
+                        f"{tuple(kcache.shape)} and {tuple(vcache.shape)}")
+    return dt, P, hkv, D
+
+
+def page_plan(ctx_lens, new_lens, page_table, num_pages, max_tokens, free_pages=None, n_free=None, out=None, status=None):
+    """Block tables, positions and slot map of a step from its request lengths (no counterpart in the reference, whose
+    engine does this on the host).  Request b holds ctx_lens[b] tokens and brings new_lens[b] (int32 [B], device);
+    page_table int32 [B, W] has the pages of the cached tokens and receives those of the new ones, taken off the end of
+    free_pages int32 [F] (of which n_free int32 [1] are valid; not changed, see `n_left`).  Without free_pages the table
+    must hold every page already.  max_tokens: rows of the step's token buffers.  Returns a `PagePlan` (`out` is
+    written in place if given); rows behind the last request have position 0 and slot -1."""
+    _need(ctx_lens, torch.int32, "ctx_lens", 1)
+    _need(new_lens, torch.int32, "new_lens", 1)
+    _need(page_table, torch.int32, "page_table", 2)
+    B, dev, T = ctx_lens.shape[0], ctx_lens.device, int(max_tokens)
+    if new_lens.shape[0] != B or page_table.shape[0] != B:
+        raise B200Error("page_plan: ctx_lens, new_lens and page_table must have one entry per request")
+    if free_pages is not None:
+        _need(free_pages, torch.int32, "free_pages", 1)
+        if n_free is None:
+            raise B200Error("page_plan: a free list needs n_free")
+        _need(n_free, torch.int32, "n_free")
+        if n_free.numel() != 1:
+            raise B200Error("page_plan: n_free must have one element")
+    _together("page_plan", dev, new_lens, page_table, free_pages, n_free)
+    _need_status("page_plan", status, dev)
+    if out is None:
+        if T <= 0 or B == 0:
+            raise B200Error(f"page_plan: need at least one request and one row (B={B} max_tokens={T})")
+        i32, i64 = dict(dtype=torch.int32, device=dev), dict(dtype=torch.int64, device=dev)
+        out = PagePlan(torch.empty(B + 1, **i32), torch.empty(B, **i32), torch.empty(T, **i64), torch.empty(T, **i64),
+                       torch.empty(1, **i32))
+    else:
+        for t, dt, n in ((out.cu_seqlens, torch.int32, B + 1), (out.seqlens, torch.int32, B), (out.positions, torch.int64, T),
+                         (out.slots, torch.int64, T), (out.n_left, torch.int32, 1)):
+            _need(t, dt, "page_plan: an output", 1)
+            if t.shape[0] != n:
+                raise B200Error("page_plan: the outputs were sized for another batch")
+        _together("page_plan", dev, *out)
+    _launch("b200_page_plan", _lib.lib().b200_page_plan, dev, ctx_lens.data_ptr(), new_lens.data_ptr(), B,
+            page_table.data_ptr(), page_table.shape[1], int(num_pages), _ptr(free_pages),
+            0 if free_pages is None else free_pages.shape[0], _ptr(n_free), T, out.cu_seqlens.data_ptr(),
+            out.seqlens.data_ptr(), out.positions.data_ptr(), out.slots.data_ptr(), out.n_left.data_ptr(), _ptr(status))
+    return out
+
+
+def kv_append(k, v, kcache, vcache, slots, status=None):
+    """New tokens' K and V (e4m3 codes as uint8, or bf16, as the caches; [T, kv heads, dim], a token stride of their own)
+    into the pages at slots int64 [T] (`PagePlan.slots`; negative: skipped).  kcache [P, kv heads, 128, dim] and vcache
+    [P, kv heads, dim, 128] are updated in place."""
+    dt, P, hkv, D = _need_pages(kcache, vcache)
+    ks = _token_rows(k, dt, "k", hkv, D)
+    vs = _token_rows(v, dt, "v", hkv, D)
+    _need(slots, torch.int64, "slots", 1)
+    T = k.shape[0]
+    if v.shape[0] != T or slots.shape[0] != T:
+        raise B200Error("kv_append: k, v and slots must have one row per token")
+    _together("kv_append", kcache.device, k, v, vcache, slots)
+    _need_status("kv_append", status, kcache.device)
+    if T == 0:
+        return
+    _launch("b200_kv_append", _lib.lib().b200_kv_append, kcache.device, k.data_ptr(), v.data_ptr(), ks, vs, T, hkv, D,
+            1 if dt == torch.bfloat16 else 0, kcache.data_ptr(), vcache.data_ptr(), P, slots.data_ptr(), _ptr(status))
+
+
+def attn_extend(q, gate, kcache, vcache, page_table, cu_seqlens, seqlens, scale=None, out=None, ws=None, status=None):
+    """Attention of ragged chunks of new tokens over the paged cache, the new tokens included (`kv_append` first); one
+    new token per request is plain decode.  q [T, heads, dim] in the caches' type, gate bf16 [T, heads, dim] or None (no
+    output gate); page_table int32 [B, W], cu_seqlens int32 [B + 1] and seqlens int32 [B] as `page_plan` leaves them:
+    row i of request b sees keys 0 .. seqlens[b] - new + i.  Rows that see no key come out as zeros, rows behind the last
+    request are left as they are.  Returns out bf16 [T, heads * dim]."""
+    dt, P, hkv, D = _need_pages(kcache, vcache)
+    qs = _token_rows(q, dt, "q", None, D)
+    T, hq = q.shape[:2]
+    gs = 0
+    if gate is not None:
+        gs = _token_rows(gate, torch.bfloat16, "gate", hq, D)
+        if gate.shape[0] != T:
+            raise B200Error("attn_extend: gate must have a row per token")
+    _need(page_table, torch.int32, "page_table", 2)
+    _need(cu_seqlens, torch.int32, "cu_seqlens", 1)
+    _need(seqlens, torch.int32, "seqlens", 1)
+    B, dev = seqlens.shape[0], q.device
+    if cu_seqlens.shape[0] != B + 1 or page_table.shape[0] != B:
+        raise B200Error("attn_extend: page_table [B, W], cu_seqlens [B + 1] and seqlens [B] do not fit together")
+    _together("attn_extend", dev, gate, kcache, vcache, page_table, cu_seqlens, seqlens, out, ws)
+    _need_status("attn_extend", status, dev)
+    if out is None:
+        out = torch.empty(T, hq * D, dtype=torch.bfloat16, device=dev)
+    else:
+        _need(out, torch.bfloat16, "out", 2)
+        if tuple(out.shape) != (T, hq * D):
+            raise B200Error("attn_extend: out must be [T, heads * dim]")
+    if T == 0:
+        return out
+    if ws is None:
+        ws = attn_extend_workspace(T, hq, hkv, D, dev)
+    else:
+        _need(ws, torch.uint8, "ws", 1)
+    _launch("b200_attn_extend", _lib.lib().b200_attn_extend, dev, q.data_ptr(), qs, _ptr(gate), gs, kcache.data_ptr(),
+            vcache.data_ptr(), P, page_table.data_ptr(), page_table.shape[1], cu_seqlens.data_ptr(), seqlens.data_ptr(), B, T,
+            hq, hkv, D, 1 if dt == torch.bfloat16 else 0, float(scale) if scale is not None else D ** -0.5, out.data_ptr(),
+            ws.data_ptr(), ws.numel(), _ptr(status))
+    return out
+
+
+def attn_extend_workspace(T, heads, kv_heads, dim, device):
+    n = _lib.lib().b200_attn_extend_workspace_bytes(T, heads, kv_heads, dim)
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
 
 
 def dense_fp8_workspace(T, H, device):

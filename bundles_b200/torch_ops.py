@@ -20,6 +20,11 @@ _lib.define("attn_front(Tensor x, Tensor w, Tensor w_s, Tensor q_norm_w, Tensor 
             "Tensor cos_sin, float eps, bool out_fp8) -> (Tensor, Tensor, Tensor, Tensor)")
 _lib.define("attn_verify(Tensor q, Tensor gate, Tensor k_new, Tensor v_new, Tensor(a!) kcache, Tensor(b!) vcache, "
             "Tensor page_table, Tensor seqlens, float scale) -> Tensor")
+_lib.define("page_plan(Tensor ctx_lens, Tensor new_lens, Tensor(a!) page_table, int num_pages, int max_tokens, "
+            "Tensor? free_pages, Tensor? n_free) -> (Tensor, Tensor, Tensor, Tensor, Tensor)")
+_lib.define("kv_append(Tensor k, Tensor v, Tensor(a!) kcache, Tensor(b!) vcache, Tensor slots) -> ()")
+_lib.define("attn_extend(Tensor q, Tensor? gate, Tensor kcache, Tensor vcache, Tensor page_table, Tensor cu_seqlens, "
+            "Tensor seqlens, float scale) -> Tensor")
 _lib.define("lmhead_argmax(Tensor x, Tensor w, Tensor w_s, int shard_lo) -> (Tensor, Tensor)")
 _lib.define("moe_combine(Tensor cache, Tensor x, Tensor? gate_w, int top_k, Tensor? pos) -> Tensor")
 _lib.define("moe_combine_norm(Tensor cache, Tensor x, Tensor? gate_w, int top_k, Tensor(a!) residual, Tensor norm_w, "
@@ -60,6 +65,18 @@ def _attn(x, w, w_s, qw, kw, positions, cos_sin, eps, out_fp8):
 
 def _attn_verify(q, gate, k_new, v_new, kcache, vcache, page_table, seqlens, scale):
     return ops.attn_verify(q, gate, k_new, v_new, kcache, vcache, page_table, seqlens, scale)
+
+
+def _page_plan(ctx_lens, new_lens, page_table, num_pages, max_tokens, free_pages, n_free):
+    return tuple(ops.page_plan(ctx_lens, new_lens, page_table, num_pages, max_tokens, free_pages, n_free))
+
+
+def _kv_append(k, v, kcache, vcache, slots):
+    ops.kv_append(k, v, kcache, vcache, slots)
+
+
+def _attn_extend(q, gate, kcache, vcache, page_table, cu_seqlens, seqlens, scale):
+    return ops.attn_extend(q, gate, kcache, vcache, page_table, cu_seqlens, seqlens, scale)
 
 
 def _lmhead(x, w, w_s, shard_lo):
@@ -149,5 +166,8 @@ _lib.impl("gdn_verify", _gdn, "CUDA")
 _lib.impl("gdn_verify_replay", _gdn_replay, "CUDA")
 _lib.impl("attn_front", _attn, "CUDA")
 _lib.impl("attn_verify", _attn_verify, "CUDA")
+_lib.impl("page_plan", _page_plan, "CUDA")
+_lib.impl("kv_append", _kv_append, "CUDA")
+_lib.impl("attn_extend", _attn_extend, "CUDA")
 _lib.impl("lmhead_argmax", _lmhead, "CUDA")
 _lib.impl("moe_combine", _combine, "CUDA")

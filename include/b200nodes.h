@@ -42,6 +42,9 @@ extern "C" {
 #define B200_ST_WAIT_STORE 106
 #define B200_ST_WAIT_PEER 107   /* expert-parallel barrier: a peer rank's flag did not arrive in time */
 #define B200_ST_BAD_LIST 110
+#define B200_ST_NO_PAGE 111     /* a token without a page: the free list ran out or the block table is too narrow */
+#define B200_ST_BAD_PAGE 112    /* a page id or slot outside the pool (skipped) */
+#define B200_ST_BAD_LEN 113     /* a negative length, or more new tokens than rows (clamped) */
 
 int b200_abi_version(void);
 const char* b200_last_error(void);
@@ -347,6 +350,50 @@ int b200_attn_verify(const void* q, const void* gate, const void* k_new, const v
                      void* vcache, int num_pages, const int32_t* page_table, int pt_stride,
                      const int32_t* seqlens, int B, float scale, int splits, void* out, void* ws,
                      size_t ws_bytes, int32_t* status, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * The paged cache for ragged batches: prompts in chunks, plain decode, and steps that mix the two.  (No counterpart in
+ * the reference's nodes: its engine builds the tables on the host, and its prefill and decode attention are library calls,
+ * attn_fused.py:158-162.)  Pages as above: 128 tokens, K [num_pages][Hkv][128 tokens][D], V [num_pages][Hkv][D][128 tokens],
+ * in e4m3 codes or (cache_bf16 != 0) bf16; D = 128 or 256.
+ *
+ * b200_page_plan: block tables, positions and slots from request lengths.  Request b has ctx_lens[b] tokens in its pages
+ * and new_lens[b] tokens in this step; its rows of the step are cu_seqlens[b] .. cu_seqlens[b + 1] - 1 in request order.
+ *   page_table int32 [B, pt_stride], in and out: the entries of the cached tokens are read, those of the new pages are
+ *     written, all others are left as they are.  New pages come off the END of free_pages [free_cap] (n_free of them are
+ *     valid) in request order, then in page order; n_left receives how many remain (n_free itself is only read).
+ *     free_pages NULL: the table holds every page already (n_free, n_left unused).
+ *   cu_seqlens int32 [B + 1]; seqlens int32 [B] = cached + new; positions, slots int64 [T]: the token's place in its
+ *     request and in the pool (page * 128 + place in the page).  Rows behind the last request: position 0, slot -1.
+ *   A token whose page is missing gets slot -1 and a table entry -1: the free list ran out or the table is too narrow
+ *     (B200_ST_NO_PAGE), an id is outside [0, num_pages) (B200_ST_BAD_PAGE).  Negative lengths count as 0 and tokens
+ *     beyond T rows are dropped (B200_ST_BAD_LEN).  B <= 8192.
+ *
+ * b200_kv_append: the new tokens' K and V, [T, Hkv, D] with token strides in elements (multiples of 16 bytes), into
+ * the pages at `slots`.  Rows with a negative slot are skipped, slots outside the pool too (B200_ST_BAD_PAGE).  No two
+ * rows may name the same slot.
+ *
+ * b200_attn_extend: the tokens' attention over their requests' pages, the new tokens included (append first): row i of
+ * request b sees keys 0 .. seqlens[b] - new + i; q head h reads kv head h / (Hq / Hkv).
+ *   out[t, h] = sigmoid(gate[t, h]) * softmax(scale * q . K) V in bf16, rounded once; gate bf16 or NULL (no gate).
+ *   q e4m3 or bf16 as the cache, [T, Hq, D] with a token stride in elements; out bf16 [T, Hq * D].
+ *   A row that sees no key is written as zeros; rows behind cu_seqlens[B] are left as they are; keys on missing pages
+ *   are masked (B200_ST_BAD_PAGE).  Keys behind a request's last token may hold anything, NaN included.
+ *   cu_seqlens[0] = 0 and ascending, seqlens >= 0.  scale > 0.
+ *   ws: b200_attn_extend_workspace_bytes(T, Hq, Hkv, D) bytes, 16-byte aligned, one per call in flight.
+ */
+int b200_page_plan(const int32_t* ctx_lens, const int32_t* new_lens, int B, int32_t* page_table, int pt_stride,
+                   int num_pages, const int32_t* free_pages, int free_cap, const int32_t* n_free, int T,
+                   int32_t* cu_seqlens, int32_t* seqlens, int64_t* positions, int64_t* slots, int32_t* n_left,
+                   int32_t* status, void* stream);
+int b200_kv_append(const void* k, const void* v, long long k_stride, long long v_stride, int T, int Hkv, int D,
+                   int cache_bf16, void* kcache, void* vcache, int num_pages, const int64_t* slots, int32_t* status,
+                   void* stream);
+size_t b200_attn_extend_workspace_bytes(int T, int Hq, int Hkv, int D);
+int b200_attn_extend(const void* q, long long q_stride, const void* gate, long long gate_stride, const void* kcache,
+                     const void* vcache, int num_pages, const int32_t* page_table, int pt_stride,
+                     const int32_t* cu_seqlens, const int32_t* seqlens, int B, int T, int Hq, int Hkv, int D,
+                     int cache_bf16, float scale, void* out, void* ws, size_t ws_bytes, int32_t* status, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Fused gated-attention projection front.  Replaces fp8.linear_q + qk_attn_verify.
