@@ -1,4 +1,26 @@
-// Attention of ragged chunks of new tokens over the paged KV cache (prompts in chunks, plain decode, mixed batches).
+// Attention of ragged chunks of new tokens over the paged KV cache: prompts in chunks, plain decode (one new token per
+// request), and steps that mix the two.  Query i of a request with n keys and m new tokens sees keys 0 .. n - m + i.
+//
+//   o = sigmoid(gate) * sum_j w_j v_j / sum_j w_j,   w_j = 2^((q . k_j - m) scale log2 e)
+//
+// in one pass over the pages: the running maximum m moves only when a page exceeds it by more than AX_TAU (log2), the row
+// sums and the accumulator are fp32, and the partial (o, m, l) of ranges that were cut are merged in page order.
+//
+// Rows.  The query heads of one kv head share its keys, so a tile's 128 rows are (token, head of the group) pairs of one
+// request: 128 / group tokens at a time.  Q . K^T and P . V run on tcgen05 with the rows on the M side; a softmax thread
+// owns one row and half of the page's 128 keys, so a row's maximum and sum need one exchange between two warps.
+//
+// P in 8 bits.  With e4m3 pages V is the B operand of an 8-bit MMA as it lies in the page, which saves the conversion
+// of V to f16 (64 KB of shared memory and three passes over it per page) and half of the tensor time of a 16-bit product
+// for each of the two terms that P is given in: an e5m2 value h of P 2^AX_BIAS and the e4m3 value of the remainder
+// P 2^AX_BIAS - h.  h is within 2^(e-3) of a probability in [2^e, 2^(e+1)) and the remainder's own rounding within
+// 2^(e-8): half a step of 2^-8, what bf16 has.  The range: the remainder is a normal number for probabilities down to
+// 2^-11 of the maximum, h alone down to 2^-22 and, as a subnormal, 2^-25.  With bf16 pages P is bf16.
+//
+// Work.  Every (kv head, request, tile) costs its pages plus AX_OVH; the sequence of all of them is cut into equal
+// ranges, one per CTA, so that a batch of any shape fills the GPU.  Every CTA finds its range from the lengths by itself
+// (a closed form for the pages of a request's first k tiles), so nothing is planned on the host and a captured graph may
+// be replayed with other lengths.
 #include "common.cuh"
 #include "host.h"
 
@@ -7,121 +29,855 @@ namespace b200 {
 B200_DEFINE_WAIT_BUDGET_SETTER(set_wait_budget_attn_extend)
 
 constexpr int AX_PAGE = 128;
+constexpr int AX_OVH = 2;              // cost of a tile beside its pages, in pages
+constexpr int AX_MIN_UNITS = 4;        // smallest range worth a CTA of its own
+constexpr float AX_BIAS = 8.f;         // log2 scale of the 8-bit probabilities
+constexpr float AX_TAU = 4.f;          // log2 distance that moves the running maximum: 2^(8 + 4) fits both formats
+constexpr int AX_ITEMS = 4;            // ring of work items
+constexpr int AX_WARPS = 12;           // K, V, MMA, scheduler, 8 softmax
+constexpr int AX_THREADS = AX_WARPS * 32;
+constexpr int AX_SOFT0 = 4, AX_SOFT = 8;
 
 struct AxArgs {
   const void* q;
   long long q_stride;
   const bf16* gate;
   long long gate_stride;
-  const void* kc;
-  const void* vc;
   int num_pages;
   const int32_t* table;
   int pt_stride;
   const int32_t* cu;
   const int32_t* seqlens;
-  int B, T, hq, hkv;
+  int B, T, hq, hkv, grp, tpt;   // grp query heads per kv head, tpt tokens per tile
   float scale_log2;
   bf16* out;
+  int32_t* desc;                 // [grid][8]: tiles to merge
+  float* part;                   // [2 * grid][rows][D] unnormalised, then [2 * grid][2][rows]: maximum, row sum
+  int rows;                      // tpt * grp
   int32_t* status;
 };
 
-__device__ __forceinline__ float ax_float(uint8_t v) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<unsigned short>(v)));
-  return __half2float(__ushort_as_half(static_cast<unsigned short>(r & 0xffffu)));
-}
-__device__ __forceinline__ float ax_float(bf16 v) { return bf2f(v); }
+// one piece of work: pages [p0, p1) of one tile
+struct AxItem {
+  int req, head, tok0, ntok;     // tok0: row of the tile's first token in q
+  int pos0, p0, p1, slot;        // pos0: its place in the request; slot: partial slot or -1
+};
 
-// One CTA per (token, kv head); heads of the group in slices of 8.
-template <typename E, int D>
-__global__ void __launch_bounds__(256) attn_extend_rows_kernel(const AxArgs p) {
-  __shared__ float s_q[8][D], s_p[8][AX_PAGE], s_a[8], s_l[8];
-  __shared__ int s_b;
+template <bool F8, int D>
+struct AxShape {
+  static constexpr int ES = F8 ? 1 : 2;
+  static constexpr int ROWB = D * ES;                  // bytes of a Q or K row
+  static constexpr int NB = ROWB / 128;                // 128-byte blocks of a row
+  static constexpr int PAGEB = AX_PAGE * ROWB;         // bytes of a K (or V) page of one kv head
+  static constexpr int UNIT = PAGEB < 32768 ? PAGEB : 32768;
+  static constexpr int PU = PAGEB / UNIT;              // ring units per page
+  static constexpr int NK = PU == 2 ? 2 : (UNIT == 16384 ? 5 : 3);   // K stages (units)
+  static constexpr int NV = PU == 2 ? 3 : (UNIT == 16384 ? 5 : 3);   // V stages
+  static constexpr int QB = NB * 16384;                // Q tile: NB blocks of [128 rows x 128 bytes]
+  static constexpr int OFF_K = QB;
+  static constexpr int OFF_V = OFF_K + NK * UNIT;
+  static constexpr int OFF_BAR = OFF_V + NV * UNIT;
+  static constexpr int OFF_ITEM = OFF_BAR + 512;   // at most 60 barriers and 24 bytes
+  static constexpr int OFF_RED = OFF_ITEM + AX_ITEMS * 32;
+  static constexpr int SMEM = OFF_RED + 2 * 2 * 128 * 4;
+  static_assert(SMEM <= 232448, "shared memory of a CTA");
+  static constexpr int VBOX = D * 128;                 // one V box: D rows of 128 bytes
+  static constexpr int NVB = ES;                       // boxes per V page
+};
+
+__device__ __forceinline__ uint32_t ax_sw128(int row, int chunk) {
+  return static_cast<uint32_t>((row >> 3) * 1024 + (row & 7) * 128 + ((chunk ^ (row & 7)) << 4));
+}
+// D += A B with A in tensor memory
+template <bool F8>
+__device__ __forceinline__ void ax_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if (F8)
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+template <bool F8>
+__device__ __forceinline__ void ax_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if (F8)
+    tc_mma_f8(d, a, b, idesc, accumulate);
+  else
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// instruction descriptor: M = 128, N = n, fp32 accumulator, K-major operands
+__device__ __forceinline__ uint32_t ax_idesc(uint32_t a_fmt, uint32_t b_fmt, uint32_t n) {
+  return (UMMA_C_F32 << 4) | (a_fmt << 7) | (b_fmt << 10) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+__device__ __forceinline__ void ax_tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void ax_tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ax_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t ax_e5m2x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// a probability rounded to three significant bits, which e5m2 holds exactly
+__device__ __forceinline__ float ax_head(float p) {
+  return __uint_as_float((__float_as_uint(p) + 0x00100000u) & 0xffe00000u);
+}
+__device__ __forceinline__ void ax_tma_load_3d(void* smem_dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(smem_u32(smem_dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// sum over i < m of floor((a + i s) / d); a, s >= 0, d > 0 (Euclid's descent on (d, s))
+__device__ __forceinline__ long long ax_floor_sum(long long m, long long d, long long s, long long a) {
+  long long r = 0;
+  while (m > 0) {
+    r += m * (a / d);
+    a %= d;
+    r += m * (m - 1) / 2 * (s / d);
+    s %= d;
+    const long long y = s * m + a;
+    if (y < d) break;
+    m = y / d;
+    a = y % d;
+    const long long t = d;
+    d = s;
+    s = t;
+  }
+  return r;
+}
+// pages that a tile reads whose last token sees keys 0 .. end - 1
+__device__ __forceinline__ int ax_pages(int end) { return end <= 0 ? 0 : (end + AX_PAGE - 1) / AX_PAGE; }
+// cost of a request's first k tiles, all of tpt tokens; ctx: keys before its first new token (negative: missing)
+__device__ __forceinline__ long long ax_cost(int k, int ctx, int tpt) {
+  const int skip = ctx < 0 ? min(k, -ctx / tpt) : 0;   // tiles whose last token sees nothing
+  return static_cast<long long>(k) * AX_OVH +
+         ax_floor_sum(k - skip, AX_PAGE, tpt, static_cast<long long>(ctx) + static_cast<long long>(skip + 1) * tpt + AX_PAGE - 1);
+}
+__device__ __forceinline__ long long ax_cost_all(int n, int ctx, int tpt) {
+  if (n <= 0) return 0;
+  return ax_cost((n - 1) / tpt, ctx, tpt) + AX_OVH + ax_pages(ctx + n);
+}
+
+// Waits of a whole warp: every lane polls, and all give up together.
+__device__ __forceinline__ bool ax_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  return __all_sync(FULL_MASK, mbar_wait(bar, parity, abort_flag, status, code));
+}
+// After an abandoned wait: gives a copy or a commit that is still in flight a bounded time.
+__device__ __forceinline__ void ax_drain(uint64_t* bar, uint32_t parity) {
+  const unsigned long long t0 = globaltimer();
+  while (!mbar_try(bar, parity) && globaltimer() - t0 < 20ull * 1000 * 1000) {
+  }
+}
+
+template <bool F8, int D>
+__global__ void __launch_bounds__(AX_THREADS, 1)
+attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                   const __grid_constant__ CUtensorMap tmV, const AxArgs p) {
+  using X = AxShape<F8, D>;
+  extern __shared__ __align__(1024) uint8_t smem[];   // the swizzled tiles start on 1024 bytes; there is no room for slack
+  if (smem_u32(smem) & 1023u) {
+    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, ST_WAIT_STATE);
+    return;
+  }
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + X::OFF_BAR);
+  uint64_t* kfull = bars;                 // [NK]
+  uint64_t* kempty = kfull + X::NK;       // [NK]
+  uint64_t* vfull = kempty + X::NK;       // [NV]
+  uint64_t* vempty = vfull + X::NV;       // [NV]
+  uint64_t* ifull = vempty + X::NV;       // [AX_ITEMS] item written
+  uint64_t* iempty = ifull + AX_ITEMS;    // [AX_ITEMS] all roles are done with it
+  uint64_t* sfull = iempty + AX_ITEMS;    // [2] scores complete in TMEM
+  uint64_t* pready = sfull + 2;           // [2] probabilities written (and O rescaled if needed)
+  uint64_t* xch = pready + 2;             // [4] the two warps of a TMEM quadrant published their halves
+  uint64_t* qfull = xch + 4;              // Q tile landed
+  uint64_t* qempty = qfull + 1;           // the item's last score MMA is done
+  uint64_t* pvdone = qempty + 1;          // P . V of a page done
+  uint64_t* ofree = pvdone + 1;           // the accumulator has been read
+  uint64_t* vtail = ofree + 1;            // [NV] V page with places behind the last key landed
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(vtail + X::NV);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* s_start = reinterpret_cast<int*>(tmem_slot + 2);   // request
+  long long* s_off = reinterpret_cast<long long*>(tmem_slot + 4);
+  AxItem* items = reinterpret_cast<AxItem*>(smem + X::OFF_ITEM);
+  float* red = reinterpret_cast<float*>(smem + X::OFF_RED);   // [2 pages][2 halves][128 rows]
+  long long* s_scan = reinterpret_cast<long long*>(smem + X::OFF_V);   // prelude only, before any copy is issued
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < X::NK; ++i) {
+      mbar_init(&kfull[i], 1);
+      mbar_init(&kempty[i], 1);
+    }
+    for (int i = 0; i < X::NV; ++i) {
+      mbar_init(&vfull[i], 1);
+      mbar_init(&vempty[i], 1);
+      mbar_init(&vtail[i], 1);
+    }
+    for (int i = 0; i < AX_ITEMS; ++i) {
+      mbar_init(&ifull[i], 1);
+      mbar_init(&iempty[i], 3 + AX_SOFT);   // K, V, MMA, softmax warps
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sfull[i], 1);
+      mbar_init(&pready[i], AX_SOFT);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(&xch[i], 2);
+    mbar_init(qfull, 1);
+    mbar_init(qempty, 1);
+    mbar_init(pvdone, 1);
+    mbar_init(ofree, AX_SOFT);
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  if (warp == 2) tmem_alloc(tmem_slot, 512);
   pdl_wait();
   pdl_launch();
-  const int t = blockIdx.x / p.hkv, h = blockIdx.x % p.hkv, grp = p.hq / p.hkv;
-  if (threadIdx.x == 0) s_b = -1;
+
+  // ---- this CTA's range of the work: every thread costs a slice of the requests, the CTA scans the slices ----
+  const int cta = blockIdx.x, grid = gridDim.x;
+  const int per = (p.B + AX_THREADS - 1) / AX_THREADS, b0 = min(p.B, static_cast<int>(threadIdx.x) * per), b1 = min(p.B, b0 + per);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int n = p.cu[b + 1] - p.cu[b];
+    mine += ax_cost_all(n, p.seqlens[b] - n, p.tpt);
+  }
+  long long inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(FULL_MASK, inc, o);
+    if (lane >= o) inc += u;
+  }
+  if (lane == 31) s_scan[warp] = inc;
+  if (threadIdx.x == 0) *s_start = -1;
   __syncthreads();
-  for (int b = threadIdx.x; b < p.B; b += 256)
-    if (p.cu[b] <= t && t < p.cu[b + 1]) s_b = b;
+  long long before = inc - mine, C = 0;
+  for (int w = 0; w < AX_WARPS; ++w) {
+    const long long v = s_scan[w];
+    if (w < warp) before += v;
+    C += v;
+  }
+  const long long U = C * p.hkv;
+  const long long n_want = (U + AX_MIN_UNITS - 1) / AX_MIN_UNITS;
+  const int n_eff = n_want > grid ? grid : static_cast<int>(n_want);
+  const long long u0 = cta < n_eff ? cta * U / n_eff : U, u1 = cta < n_eff ? (cta + 1) * U / n_eff : U;
+  if (u0 < u1) {
+    const long long v0 = u0 % C;
+    if (v0 >= before && v0 < before + mine) {
+      long long at = before;
+      for (int b = b0; b < b1; ++b) {
+        const int n = p.cu[b + 1] - p.cu[b];
+        const long long c = ax_cost_all(n, p.seqlens[b] - n, p.tpt);
+        if (v0 < at + c) {
+          *s_start = b;
+          *s_off = v0 - at;
+          break;
+        }
+        at += c;
+      }
+    }
+  }
+  fence_proxy_async();
+  tc_fence_before();
   __syncthreads();
-  const int b = s_b;
-  if (b < 0) return;
-  const int n = p.seqlens[b] - (p.cu[b + 1] - p.cu[b]) + (t - p.cu[b]) + 1;   // keys that this token sees
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const E* kc = static_cast<const E*>(p.kc);
-  const E* vc = static_cast<const E*>(p.vc);
-  for (int g0 = 0; g0 < grp; g0 += 8) {
-    const int ng = min(8, grp - g0);
-    for (int i = threadIdx.x; i < ng * D; i += 256)
-      s_q[i / D][i % D] = ax_float(static_cast<const E*>(p.q)[t * p.q_stride + (h * grp + g0 + i / D) * D + i % D]) * p.scale_log2;
-    float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;   // m, l: head `warp`, in every lane
-    for (int k0 = 0; k0 < n; k0 += AX_PAGE) {
-      const int j = k0 / AX_PAGE;
-      const int page = j < p.pt_stride ? p.table[static_cast<size_t>(b) * p.pt_stride + j] : -1;
-      if (page < 0 || page >= p.num_pages) {
-        if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, B200_ST_BAD_PAGE);
-        continue;
-      }
-      __syncthreads();
-      const size_t ph = static_cast<size_t>(page) * p.hkv + h;
-      for (int key = warp; key < AX_PAGE; key += 8) {
-        float acc[8] = {};
-        for (int d = lane; d < D; d += 32) {
-          const float kv = ax_float(kc[(ph * AX_PAGE + key) * D + d]);
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t TM_O = tmem, TM_S = tmem + 256;   // O: D columns; two score buffers of 128 columns
+
+  // items in order; `it` counts them
+  auto item_wait = [&](int it, AxItem& x) -> bool {
+    if (!ax_wait(&ifull[it % AX_ITEMS], (it / AX_ITEMS) & 1, abort_flag, p.status, ST_WAIT_FULL)) return false;
+    x = items[it % AX_ITEMS];
+    return x.p1 > x.p0;    // an empty item ends the list
+  };
+  auto item_done = [&](int it) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&iempty[it % AX_ITEMS]);
+  };
+
+  if (warp == 3) {
+    // ---------------- scheduler: walks the tiles of this CTA's range.  The same warp clears, in the copy of the last V page
+    // of an item, the places behind the last key that its tile sees: they may hold anything, and a zero probability
+    // times a NaN would spoil the row.  Such a page lands on a barrier of its own and counts as full once it is cleared.
+    // An item is cleared before its place in the ring is waited for, so neither duty holds up the other ----------------
+    int it = 0, cl = 0, pages = 0;   // items written, items cleared, pages of the cleared ones
+    uint32_t tails = 0;              // per stage: phase of its tail barrier
+    bool ok = true, described = false;
+    auto clear = [&]() -> bool {
+      const AxItem x = items[cl % AX_ITEMS];
+      const int last = x.pos0 + x.ntok - (x.p1 - 1) * AX_PAGE;
+      ++cl;
+      pages += x.p1 - x.p0;
+      if (last >= AX_PAGE) return true;
+      for (int u = 0; u < X::PU; ++u) {
+        const int un = (pages - 1) * X::PU + u, st = un % X::NV;
+        if (!ax_wait(&vtail[st], (tails >> st) & 1, abort_flag, p.status, ST_WAIT_FULL)) return false;
+        tails ^= 1u << st;
+        for (int c = 0; c < X::UNIT / X::VBOX; ++c) {
+          const int vb = min(128, max(0, last * X::ES - (u * (X::UNIT / X::VBOX) + c) * 128));   // valid bytes of a row of the box
+          uint8_t* box = smem + X::OFF_V + st * X::UNIT + c * X::VBOX;
+          for (int d = lane; d < D; d += 32)
+            for (int ch = vb >> 4; ch < 8; ++ch) {
+              uint32_t* w = reinterpret_cast<uint32_t*>(box + ax_sw128(d, ch));
 #pragma unroll
-          for (int g = 0; g < 8; ++g)
-            if (g < ng) acc[g] = fmaf(kv, s_q[g][d], acc[g]);
+              for (int e = 0; e < 4; ++e) {
+                const int keep = vb - ch * 16 - e * 4;         // bytes of this word that are valid
+                if (keep <= 0)
+                  w[e] = 0;
+                else if (keep < 4)
+                  w[e] &= 0xffffffffu >> (32 - keep * 8);
+              }
+            }
         }
-#pragma unroll
-        for (int g = 0; g < 8; ++g) {
-          for (int x = 16; x > 0; x >>= 1) acc[g] += __shfl_xor_sync(FULL_MASK, acc[g], x);
-          if (lane == g) s_p[g][key] = k0 + key < n ? acc[g] : -INFINITY;
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&vfull[st]);
+      }
+      return true;
+    };
+    auto push = [&](const AxItem& x) -> bool {
+      const int s = it % AX_ITEMS;
+      if (it >= AX_ITEMS && !clear()) return false;
+      if (!ax_wait(&iempty[s], ((it / AX_ITEMS) & 1) ^ 1u, abort_flag, p.status, ST_WAIT_EMPTY)) return false;
+      if (lane == 0) {
+        items[s] = x;
+        mbar_arrive(&ifull[s]);
+      }
+      __syncwarp();
+      ++it;
+      return true;
+    };
+    if (u0 < u1) {
+      int head = static_cast<int>(u0 / C), b = *s_start, base = -32;
+      long long off = *s_off, u = u0 - off;      // u: where the request's tiles begin
+      int w_lo = 0, w_n = 0, w_sl = 0;           // a window of 32 requests, one per lane
+      while (ok && u < u1) {
+        if (b >= p.B) {
+          b = 0;
+          ++head;
+        }
+        if (b < base || b >= base + 32 || base < 0) {
+          base = b;
+          const int r = min(b + lane, p.B - 1);
+          w_lo = p.cu[r];
+          w_n = b + lane < p.B ? p.cu[r + 1] - w_lo : 0;
+          w_sl = p.seqlens[r];
+        }
+        const int lo = __shfl_sync(FULL_MASK, w_lo, b - base), n = __shfl_sync(FULL_MASK, w_n, b - base);
+        const int ctx = __shfl_sync(FULL_MASK, w_sl, b - base) - n;
+        if (n <= 0) {
+          ++b;
+          continue;
+        }
+        const int tiles = (n + p.tpt - 1) / p.tpt;
+        int k = 0;
+        if (off > 0) {                           // the first tile whose range reaches past `off`: 32 candidates a round
+          int span = tiles;
+          while (span > 1) {
+            const int step = (span + 31) / 32;
+            const bool under = lane * step < span && ax_cost(k + lane * step, ctx, p.tpt) <= off;
+            const int l = 31 - __clz(__ballot_sync(FULL_MASK, under));
+            k += l * step;
+            span = min(step, span - l * step);
+          }
+        }
+        long long ts = u + (off > 0 ? ax_cost(k, ctx, p.tpt) : 0);
+        off = 0;
+        for (; ok && k < tiles && ts < u1; ++k) {
+          const int nt = min(p.tpt, n - k * p.tpt), end = ctx + k * p.tpt + nt, pg = ax_pages(end);
+          const long long fp = ts + AX_OVH, te = fp + pg;
+          if (pg == 0) {
+            if (ts >= u0)                        // nobody sees anything: zero rows, written by the range that has the start
+              for (int r = 0; r < nt; ++r) {
+                uint4* o = reinterpret_cast<uint4*>(p.out + (static_cast<long long>(lo + k * p.tpt + r) * p.hq + head * p.grp) * D);
+                if (lo + k * p.tpt + r < p.T)
+                  for (int c = lane; c < p.grp * D / 8; c += 32) o[c] = make_uint4(0, 0, 0, 0);
+              }
+          } else {
+            const long long a = max(fp, u0), z = min(te, u1);
+            if (a < z) {
+              AxItem x;
+              x.req = b;
+              x.head = head;
+              x.tok0 = lo + k * p.tpt;
+              x.ntok = nt;
+              x.pos0 = ctx + k * p.tpt;
+              x.p0 = static_cast<int>(a - fp);
+              x.p1 = static_cast<int>(z - fp);
+              x.slot = x.p0 == 0 ? (x.p1 == pg ? -1 : 2 * cta + 1) : 2 * cta;
+              if (x.p0 > 0 && ((fp + 1) * n_eff - 1) / U == cta - 1) {   // the first cut of its tile: merged in this CTA's name
+                described = true;
+                if (lane == 0) {
+                  int32_t* d = p.desc + cta * 8;
+                  d[0] = static_cast<int>((te * n_eff - 1) / U) - cta + 2;   // pieces
+                  d[1] = x.tok0;
+                  d[2] = nt;
+                  d[3] = head;
+                }
+              }
+              ok = push(x);
+            }
+          }
+          ts = te;
+        }
+        u = ts;
+        ++b;
+      }
+    }
+    if (!described && lane == 0) p.desc[cta * 8] = 0;
+    if (ok) {
+      AxItem end{};
+      ok = push(end);
+      while (ok && cl < it - 1) ok = clear();
+    }
+  } else if (warp == 0) {
+    // ---------------- K pages and Q tiles ----------------
+    AxItem x;
+    int un = 0, issued = 0;        // K units
+    bool ok = true;
+    int it = 0;
+    for (; ok && item_wait(it, x); ++it) {
+      if (it > 0) ok = ax_wait(qempty, (it - 1) & 1, abort_flag, p.status, ST_WAIT_EMPTY);
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_expect_tx(qfull, X::NB * p.rows * 128);
+        for (int c = 0; c < X::NB; ++c) ax_tma_load_3d(smem + c * 16384, &tmQ, c * 128, x.head * p.grp, x.tok0, qfull);
+      }
+      int ids = 0;
+      for (int j = x.p0; ok && j < x.p1; ++j) {
+        if (((j - x.p0) & 31) == 0) {
+          const int e = j + lane;
+          ids = e < x.p1 && e < p.pt_stride ? p.table[static_cast<size_t>(x.req) * p.pt_stride + e] : -1;
+          if (e < x.p1 && (ids < 0 || ids >= p.num_pages)) {
+            if (p.status) atomicCAS(p.status, 0, B200_ST_BAD_PAGE);
+            ids = p.num_pages;     // behind the pool: the copy fills zeros
+          }
+        }
+        const int id = __shfl_sync(FULL_MASK, ids, (j - x.p0) & 31);
+        const int y = id >= p.num_pages ? p.num_pages * p.hkv * AX_PAGE : (id * p.hkv + x.head) * AX_PAGE;
+        for (int u = 0; u < X::PU; ++u, ++un) {
+          const int st = un % X::NK;
+          ok = ax_wait(&kempty[st], ((un / X::NK) & 1) ^ 1u, abort_flag, p.status, ST_WAIT_EMPTY);
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_expect_tx(&kfull[st], X::UNIT);
+            for (int c = 0; c < X::UNIT / 16384; ++c)
+              tma_load_2d(smem + X::OFF_K + st * X::UNIT + c * 16384, &tmK, (u * (X::UNIT / 16384) + c) * 128, y, &kfull[st]);
+          }
+          issued = un + 1;
         }
       }
-      __syncthreads();
-      if (warp < ng) {
-        float mx = m;
-        for (int c = lane; c < AX_PAGE; c += 32) mx = fmaxf(mx, s_p[warp][c]);
-        for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(FULL_MASK, mx, x));
-        const float a = exp2f(m - mx);
-        float s = 0.f;
-        for (int c = lane; c < AX_PAGE; c += 32) {
-          const float e = exp2f(s_p[warp][c] - mx);
-          s_p[warp][c] = e;
-          s += e;
+      if (ok) item_done(it);
+    }
+    if (*abort_flag && lane == 0) {
+      for (int i = max(0, issued - X::NK); i < issued; ++i) ax_drain(&kfull[i % X::NK], (i / X::NK) & 1);
+      ax_drain(qfull, it & 1);
+    }
+  } else if (warp == 1) {
+    // ---------------- V pages ----------------
+    AxItem x;
+    int un = 0, issued = 0;
+    bool ok = true;
+    for (int it = 0; ok && item_wait(it, x); ++it) {
+      int ids = 0;
+      for (int j = x.p0; ok && j < x.p1; ++j) {
+        if (((j - x.p0) & 31) == 0) {
+          const int e = j + lane;
+          ids = e < x.p1 && e < p.pt_stride ? p.table[static_cast<size_t>(x.req) * p.pt_stride + e] : -1;
         }
-        for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(FULL_MASK, s, x);
-        l = l * a + s;
-        m = mx;
-        if (lane == 0) s_a[warp] = a;
+        const int id = __shfl_sync(FULL_MASK, ids, (j - x.p0) & 31);
+        const int y = id < 0 || id >= p.num_pages ? p.num_pages * p.hkv * D : (id * p.hkv + x.head) * D;
+        uint64_t* full = x.pos0 + x.ntok < (j + 1) * AX_PAGE ? vtail : vfull;   // keys of the page end before it does
+        for (int u = 0; u < X::PU; ++u, ++un) {
+          const int st = un % X::NV;
+          ok = ax_wait(&vempty[st], ((un / X::NV) & 1) ^ 1u, abort_flag, p.status, ST_WAIT_EMPTY);
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_expect_tx(&full[st], X::UNIT);
+            for (int c = 0; c < X::UNIT / X::VBOX; ++c)
+              tma_load_2d(smem + X::OFF_V + st * X::UNIT + c * X::VBOX, &tmV, (u * (X::UNIT / X::VBOX) + c) * 128, y, &full[st]);
+          }
+          issued = un + 1;
+        }
       }
-      __syncthreads();
-      if (threadIdx.x < D) {
-        const int d = threadIdx.x;
+      if (ok) item_done(it);
+    }
+    if (*abort_flag && lane == 0)   // a page on its tail barrier never counts as full now: its time runs out instead
+      for (int i = max(0, issued - X::NV); i < issued; ++i) ax_drain(&vfull[i % X::NV], (i / X::NV) & 1);
+  } else if (warp == 2) {
+    // ---------------- MMA issuer.  The score MMAs run two pages ahead of the P . V MMAs (also into the next item), so the
+    // tensor pipe has a product to do while the softmax warps work on a page ----------------
+    if (lane == 0) {
+      const uint32_t q_base = smem_u32(smem), k_base = smem_u32(smem + X::OFF_K), v_base = smem_u32(smem + X::OFF_V);
+      const uint32_t id_s = ax_idesc(F8 ? 0u : 1u, F8 ? 0u : 1u, 128);
+      const uint32_t id_hi = ax_idesc(1u, F8 ? 0u : 1u, D);     // P: e5m2 or bf16 (both 1); V: e4m3 0 or bf16 1
+      const uint32_t id_lo = ax_idesc(0u, 0u, D);
+      auto get = [&](int it, int& n) -> bool {       // pages of item `it`
+        if (!mbar_wait(&ifull[it % AX_ITEMS], (it / AX_ITEMS) & 1, abort_flag, p.status, ST_WAIT_FULL)) return false;
+        n = items[it % AX_ITEMS].p1 - items[it % AX_ITEMS].p0;
+        return n > 0;
+      };
+      int s_it = 0, s_i = 0, s_n = 0, ts = 0;
+      bool s_more = true, ok = true;
+      auto issue_s = [&]() {
+        if (!s_more) return;
+        if (s_i == s_n) {
+          if (!get(s_it, s_n)) {
+            s_more = false;
+            return;
+          }
+          s_i = 0;
+          if (!mbar_wait(qfull, s_it & 1, abort_flag, p.status, ST_WAIT_FULL)) {
+            s_more = ok = false;
+            return;
+          }
+          ++s_it;
+        }
+        const uint32_t d = TM_S + (ts & 1) * 128;
+        for (int u = 0; u < X::PU; ++u) {
+          const int un = ts * X::PU + u, st = un % X::NK;
+          if (!mbar_wait(&kfull[st], (un / X::NK) & 1, abort_flag, p.status, ST_WAIT_FULL)) {
+            s_more = ok = false;
+            return;
+          }
+          tc_fence_after();
 #pragma unroll
-        for (int g = 0; g < 8; ++g)
-          if (g < ng) o[g] *= s_a[g];
-        for (int c = 0; c < min(AX_PAGE, n - k0); ++c) {
-          const float vv = ax_float(vc[(ph * D + d) * AX_PAGE + c]);
+          for (int kk = 0; kk < X::UNIT / 16384 * 4; ++kk) {     // 32 bytes of a row per step, four steps per 128-byte block
+            const int c = kk >> 2;
+            ax_mma_ss<F8>(d, umma_desc_sw128(q_base + (u * (X::UNIT / 16384) + c) * 16384 + (kk & 3) * 32),
+                          umma_desc_sw128(k_base + st * X::UNIT + c * 16384 + (kk & 3) * 32), id_s, (u | kk) != 0);
+          }
+          tc_commit(&kempty[st]);
+        }
+        tc_commit(&sfull[ts & 1]);
+        ++ts;
+        if (++s_i == s_n) tc_commit(qempty);
+      };
+      issue_s();
+      issue_s();
+      int it = 0, tp = 0, n = 0;
+      while (ok && get(it, n)) {
+        for (int i = 0; ok && i < n; ++i, ++tp) {
+          const int b = tp & 1;
+          ok = mbar_wait(&pready[b], (tp >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
+          if (ok && i == 0 && it > 0) ok = mbar_wait(ofree, (it - 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY);
+          if (!ok) break;
+          const uint32_t pa = TM_S + b * 128;
+          for (int u = 0; u < X::PU; ++u) {
+            const int un = tp * X::PU + u, st = un % X::NV;
+            ok = mbar_wait(&vfull[st], (un / X::NV) & 1, abort_flag, p.status, ST_WAIT_FULL);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t vb = v_base + st * X::UNIT;
+            if (F8) {
 #pragma unroll
-          for (int g = 0; g < 8; ++g)
-            if (g < ng) o[g] = fmaf(s_p[g][c], vv, o[g]);
+              for (int kk = 0; kk < 4; ++kk)                     // 32 keys a step; the value, then the remainder
+                ax_mma_ts<F8>(TM_O, pa + kk * 8, umma_desc_sw128(vb + kk * 32), id_hi, (i | kk) != 0);
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk) ax_mma_ts<F8>(TM_O, pa + 32 + kk * 8, umma_desc_sw128(vb + kk * 32), id_lo, 1);
+            } else {
+#pragma unroll
+              for (int kk = 0; kk < 8 / X::PU; ++kk)             // 16 keys a step, four steps per box of 64 keys
+                ax_mma_ts<F8>(TM_O, pa + (u * (8 / X::PU) + kk) * 8, umma_desc_sw128(vb + (kk >> 2) * X::VBOX + (kk & 3) * 32),
+                              id_hi, (i | u | kk) != 0);
+            }
+            tc_commit(&vempty[st]);
+          }
+          if (!ok) break;
+          tc_commit(pvdone);
+          if (i == n - 1) mbar_arrive(&iempty[it % AX_ITEMS]);
+          issue_s();
+        }
+        ++it;
+      }
+      if (*abort_flag) {   // let the MMAs in flight finish before the accumulators are given back
+        tc_commit(qempty);
+        const unsigned long long t0 = globaltimer();
+        while (globaltimer() - t0 < 1000ull * 1000) {
         }
       }
     }
-    if (lane == 0) s_l[warp] = l;
-    __syncthreads();
-    if (threadIdx.x < D)
-      for (int g = 0; g < ng; ++g) {
-        const long long c = static_cast<long long>(h * grp + g0 + g) * D + threadIdx.x;
-        float r = s_l[g] == 0.f ? 0.f : o[g] / s_l[g];
-        if (p.gate) r = r / (1.f + __expf(-bf2f(p.gate[t * p.gate_stride + c])));
-        p.out[static_cast<long long>(t) * p.hq * D + c] = f2bf(r);
+  } else {
+    // ---------------- softmax: TMEM quadrant q holds rows 32 q ..; of the page's 128 keys warp 4 + q takes 0..63, warp 8 + q
+    // 64..127 ----------------
+    const int q = warp & 3, hf = (warp - AX_SOFT0) >> 2;
+    const int row = q * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
+    const float sl2 = p.scale_log2;
+    const int r_tok = row / p.grp, r_head = row - r_tok * p.grp;
+    AxItem x;
+    int tp = 0;
+    uint32_t xp = 0;                 // phase of this quadrant's exchange barrier
+    bool ok = true;
+    for (int it = 0; ok && item_wait(it, x); ++it) {
+      const int n = x.p1 - x.p0;
+      const bool active = q * 32 < x.ntok * p.grp;   // warps without a row only take part in the hand-overs
+      const bool mine_row = r_tok < x.ntok;
+      const int lim = x.pos0 + r_tok;                // last key that this row sees
+      float m = -INFINITY, l = 0.f;
+      const int32_t* tab = p.table + static_cast<size_t>(x.req) * p.pt_stride;
+      int id_next = x.p0 < p.pt_stride ? tab[x.p0] : -1;
+      for (int i = 0; ok && i < n; ++i, ++tp) {
+        const int b = tp & 1, pg = x.p0 + i;
+        const int id = id_next;
+        if (i + 1 < n) id_next = pg + 1 < p.pt_stride ? tab[pg + 1] : -1;
+        ok = ax_wait(&sfull[b], (tp >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
+        if (!ok) break;
+        if (active) {
+          tc_fence_after();
+          uint32_t s[64];
+          tmem_ld32(TM_S + b * 128 + hf * 64 + lanes, *reinterpret_cast<uint32_t(*)[32]>(s));
+          tmem_ld32(TM_S + b * 128 + hf * 64 + 32 + lanes, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
+          tmem_ld_wait();
+          const bool bad = id < 0 || id >= p.num_pages;
+          if (bad || pg * AX_PAGE + AX_PAGE - 1 > x.pos0) {      // not every row sees the whole page
+            const int see = bad ? -1 : lim - (pg * AX_PAGE + hf * 64);
+#pragma unroll
+            for (int j = 0; j < 64; ++j)
+              if (j > see) s[j] = 0xff800000u;
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int j = 0; j < 64; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(s[j]));
+          const float part = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          red[(b * 2 + hf) * 128 + row] = part;
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&xch[q]);
+          ok = ax_wait(&xch[q], xp & 1, abort_flag, p.status, ST_WAIT_STATE);
+          ++xp;
+          if (!ok) break;
+          tc_fence_after();
+          const float tm = fmaxf(part, red[(b * 2 + (hf ^ 1)) * 128 + row]);
+          const bool move = (tm - m) * sl2 > AX_TAU;             // m = -inf: any finite maximum; both -inf: NaN, no move
+          if (__any_sync(FULL_MASK, move)) {
+            const float alpha = move ? ax_exp2((m - tm) * sl2) : 1.f;
+            if (move) m = tm;
+            l *= alpha;
+            if (i > 0) {                                         // (the scores of page tp came after P . V of page tp - 2)
+              ok = ax_wait(pvdone, (tp - 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY);
+              if (!ok) break;
+              tc_fence_after();
+#pragma unroll
+              for (int c = 0; c < D / 64; ++c) {                 // this warp's half of the accumulator's columns
+                uint32_t v[32];
+                const uint32_t col = TM_O + hf * (D / 2) + c * 32 + lanes;
+                tmem_ld32(col, v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
+                ax_tmem_st16(col, v);
+                ax_tmem_st16(col + 16, v + 16);
+              }
+              ax_tmem_st_wait();
+            }
+          }
+          const float shift = (F8 ? AX_BIAS : 0.f) - (m == -INFINITY ? 0.f : m * sl2);
+          float acc[4] = {0.f, 0.f, 0.f, 0.f};
+          if (F8) {
+            uint32_t hi[16], lo[16];
+#pragma unroll
+            for (int w = 0; w < 16; ++w) {
+              float e[4], h[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                e[j] = ax_exp2(fmaf(__uint_as_float(s[w * 4 + j]), sl2, shift));
+                acc[j] += e[j];
+                h[j] = ax_head(e[j]);
+              }
+              hi[w] = ax_e5m2x2(h[0], h[1]) | (ax_e5m2x2(h[2], h[3]) << 16);
+              lo[w] = e4m3x4(e[0] - h[0], e[1] - h[1], e[2] - h[2], e[3] - h[3]);
+            }
+            ax_tmem_st16(TM_S + b * 128 + hf * 16 + lanes, hi);
+            ax_tmem_st16(TM_S + b * 128 + 32 + hf * 16 + lanes, lo);
+          } else {
+            uint32_t w16[32];
+#pragma unroll
+            for (int w = 0; w < 32; ++w) {
+              const float e0 = ax_exp2(fmaf(__uint_as_float(s[w * 2]), sl2, shift));
+              const float e1 = ax_exp2(fmaf(__uint_as_float(s[w * 2 + 1]), sl2, shift));
+              w16[w] = pack_bf2(e0, e1);
+              acc[w & 1] += bf_lo(w16[w]);        // the row sum takes the rounded values: a common error cancels
+              acc[2 + (w & 1)] += bf_hi(w16[w]);
+            }
+            ax_tmem_st16(TM_S + b * 128 + hf * 32 + lanes, w16);
+            ax_tmem_st16(TM_S + b * 128 + hf * 32 + 16 + lanes, w16 + 16);
+          }
+          ax_tmem_st_wait();
+          l += (acc[0] + acc[1]) + (acc[2] + acc[3]);
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pready[b]);
       }
-    __syncthreads();
+      if (!ok) break;
+      // ---- epilogue: the row sum's halves meet, each warp writes its half of the columns of its rows ----
+      // P . V of the page before the last may still be running (its scores came first); its phase must be over before the
+      // last page's can be told from the one before it
+      if (tp >= 2) ok = ax_wait(pvdone, tp & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
+      ok = ok && ax_wait(pvdone, (tp - 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
+      if (!ok) break;
+      if (active) {
+        tc_fence_after();
+        red[(((tp - 1) & 1) * 2 + hf) * 128 + row] = l;    // the last page's buffer: everybody has read it
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&xch[q]);
+        ok = ax_wait(&xch[q], xp & 1, abort_flag, p.status, ST_WAIT_STATE);
+        ++xp;
+        if (!ok) break;
+        const float total = l + red[(((tp - 1) & 1) * 2 + (hf ^ 1)) * 128 + row];
+        const bool store = mine_row && x.tok0 + r_tok < p.T;
+        const long long tok = x.tok0 + r_tok;
+        const int col0 = hf * (D / 2);
+        const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+        bf16* o = p.out + (tok * p.hq + x.head * p.grp + r_head) * D + col0;
+        const bf16* g = p.gate ? p.gate + tok * p.gate_stride + (x.head * p.grp + r_head) * D + col0 : nullptr;
+        float* po = p.part + (static_cast<size_t>(max(x.slot, 0)) * p.rows + row) * D + col0;
+#pragma unroll 1
+        for (int c = 0; c < D / 64; ++c) {
+          uint32_t v[32];
+          tmem_ld32(TM_O + col0 + c * 32 + lanes, v);
+          tmem_ld_wait();
+          if (store && x.slot >= 0) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              reinterpret_cast<uint4*>(po + c * 32)[j] = make_uint4(v[j * 4], v[j * 4 + 1], v[j * 4 + 2], v[j * 4 + 3]);
+          } else if (store) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              float f[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(v[j * 8 + e]) * inv;
+              if (g) {
+                const uint4 gv = reinterpret_cast<const uint4*>(g + c * 32)[j];
+                const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  f[e * 2] = __fdividef(f[e * 2], 1.f + __expf(-bf_lo(gw[e])));
+                  f[e * 2 + 1] = __fdividef(f[e * 2 + 1], 1.f + __expf(-bf_hi(gw[e])));
+                }
+              }
+              reinterpret_cast<uint4*>(o + c * 32)[j] =
+                  make_uint4(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]), pack_bf2(f[4], f[5]), pack_bf2(f[6], f[7]));
+            }
+          }
+          __syncwarp();
+        }
+        if (x.slot >= 0 && store && hf == 0) {
+          float* ml = p.part + static_cast<size_t>(2 * grid) * p.rows * D + static_cast<size_t>(x.slot) * 2 * p.rows;
+          ml[row] = m * sl2;
+          ml[p.rows + row] = total;
+        }
+        tc_fence_before();
+      }
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(ofree);
+        mbar_arrive(&iempty[it % AX_ITEMS]);
+      }
+    }
   }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Merge of the tiles whose pages were cut: the pieces are added in page order with weights 2^(m - M).  One CTA per (range
+// that a cut tile's second piece belongs to, 8 rows), one warp per row.
+template <int D>
+__global__ void __launch_bounds__(256) attn_extend_merge_kernel(const AxArgs p, int grid) {
+  pdl_wait();
+  pdl_launch();
+  const int32_t* d = p.desc + blockIdx.x * 8;
+  const int pieces = d[0];
+  if (pieces <= 0) return;
+  const int tok0 = d[1], ntok = d[2], head = d[3];
+  const int row = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int tok = tok0 + row / p.grp;
+  if (row >= ntok * p.grp || tok >= p.T) return;
+  const int first = 2 * (static_cast<int>(blockIdx.x) - 1) + 1;      // then 2 * blockIdx.x, 2 * (blockIdx.x + 1), ...
+  auto slot = [&](int i) -> size_t { return i == 0 ? first : 2 * (blockIdx.x + i - 1); };
+  const float* ml = p.part + static_cast<size_t>(2 * grid) * p.rows * D;
+  float M = -INFINITY;
+  for (int i = lane; i < pieces; i += 32) M = fmaxf(M, ml[slot(i) * 2 * p.rows + row]);
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(FULL_MASK, M, o));
+  constexpr int V = D / 128;      // float4 per lane
+  float4 acc[V] = {};
+  float L = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < pieces; ++i) {
+    const size_t s = slot(i);
+    const float m = ml[s * 2 * p.rows + row];
+    const float w = m == -INFINITY ? 0.f : ax_exp2(m - M);
+    L = fmaf(ml[s * 2 * p.rows + p.rows + row], w, L);
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      const float4 v = reinterpret_cast<const float4*>(p.part + (s * p.rows + row) * D)[c * 32 + lane];
+      acc[c].x = fmaf(v.x, w, acc[c].x);
+      acc[c].y = fmaf(v.y, w, acc[c].y);
+      acc[c].z = fmaf(v.z, w, acc[c].z);
+      acc[c].w = fmaf(v.w, w, acc[c].w);
+    }
+  }
+  const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+  const int hd = head * p.grp + row % p.grp;
+#pragma unroll
+  for (int c = 0; c < V; ++c) {
+    const int col = (c * 32 + lane) * 4;
+    float f[4] = {acc[c].x * inv, acc[c].y * inv, acc[c].z * inv, acc[c].w * inv};
+    if (p.gate) {
+      const uint2 g = *reinterpret_cast<const uint2*>(p.gate + tok * p.gate_stride + static_cast<long long>(hd) * D + col);
+      f[0] = __fdividef(f[0], 1.f + __expf(-bf_lo(g.x)));
+      f[1] = __fdividef(f[1], 1.f + __expf(-bf_hi(g.x)));
+      f[2] = __fdividef(f[2], 1.f + __expf(-bf_lo(g.y)));
+      f[3] = __fdividef(f[3], 1.f + __expf(-bf_hi(g.y)));
+    }
+    *reinterpret_cast<uint2*>(p.out + (static_cast<long long>(tok) * p.hq + hd) * D + col) =
+        make_uint2(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]));
+  }
+}
+
+template <bool F8, int D>
+static void ax_launch(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV, const AxArgs& a, cudaStream_t st) {
+  using X = AxShape<F8, D>;
+  static DeviceOnce once;
+  once.run([] { cudaFuncSetAttribute(attn_extend_kernel<F8, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, X::SMEM); });
+  const int grid = sm_count();
+  launch_k(attn_extend_kernel<F8, D>, dim3(grid), dim3(AX_THREADS), X::SMEM, st, tmQ, tmK, tmV, a);
+  launch_k(attn_extend_merge_kernel<D>, dim3(grid, (a.rows + 7) / 8), dim3(256), 0, st, a, grid);
+}
+
+// rows of a tile: the group's heads of as many tokens as fit 128 rows, or of all T
+static int ax_tokens_per_tile(int T, int grp) {
+  const int tpt = 128 / grp;
+  return T < tpt ? T : tpt;
 }
 
 }  // namespace b200
@@ -129,8 +885,9 @@ __global__ void __launch_bounds__(256) attn_extend_rows_kernel(const AxArgs p) {
 using namespace b200;
 
 extern "C" size_t b200_attn_extend_workspace_bytes(int T, int Hq, int Hkv, int D) {
-  if (T <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0) return 0;
-  return 16;
+  if (T <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || Hq % Hkv || Hq / Hkv > 128) return 0;
+  const size_t rows = static_cast<size_t>(ax_tokens_per_tile(T, Hq / Hkv)) * (Hq / Hkv), grid = sm_count();
+  return grid * 32 + 2 * grid * rows * (static_cast<size_t>(D) + 2) * 4;
 }
 
 extern "C" int b200_attn_extend(const void* q, long long q_stride, const void* gate, long long gate_stride,
@@ -146,7 +903,7 @@ extern "C" int b200_attn_extend(const void* q, long long q_stride, const void* g
   if (Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq / Hkv > 128 || Hkv > 128 || (D != 128 && D != 256))
     return fail(B200_E_ARG, "b200_attn_extend: need Hq a multiple of Hkv, at most 128 heads per group, D 128 or 256 "
                 "(Hq=%d Hkv=%d D=%d)", Hq, Hkv, D);
-  if (static_cast<long long>(num_pages) * Hkv * D > 0x7fffffffll)
+  if (static_cast<long long>(num_pages) * Hkv * D > 0x7fffff00ll)
     return fail(B200_E_ARG, "b200_attn_extend: num_pages * Hkv * D must stay below 2^31 (%d pages)", num_pages);
   if (!(scale > 0.f) || !(scale < 1e30f)) return fail(B200_E_ARG, "b200_attn_extend: scale must be positive and finite");
   const long long row = static_cast<long long>(Hq) * D, es = cache_bf16 ? 2 : 1;
@@ -159,16 +916,41 @@ extern "C" int b200_attn_extend(const void* q, long long q_stride, const void* g
   if (ws_bytes < b200_attn_extend_workspace_bytes(T, Hq, Hkv, D))
     return fail(B200_E_WS, "b200_attn_extend: workspace %zu < %zu bytes", ws_bytes,
                 b200_attn_extend_workspace_bytes(T, Hq, Hkv, D));
-  const AxArgs a{q, q_stride, static_cast<const bf16*>(gate), gate_stride, kcache, vcache, num_pages, page_table, pt_stride,
-                 cu_seqlens, seqlens, B, T, Hq, Hkv, scale * 1.4426950408889634f, static_cast<bf16*>(out), status};
+  CUtensorMap tmQ, tmK, tmV;
+  int rc;
+  AxArgs a{};
+  a.grp = Hq / Hkv;
+  a.tpt = ax_tokens_per_tile(T, a.grp);
+  a.rows = a.tpt * a.grp;
+  if ((rc = make_tmap_bytes_3d(&tmQ, q, static_cast<uint64_t>(D) * es, Hq, T, static_cast<uint64_t>(D) * es,
+                               static_cast<uint64_t>(q_stride) * es, a.grp, a.tpt, "q")))
+    return rc;
+  if ((rc = make_tmap_bytes_2d(&tmK, kcache, static_cast<uint64_t>(num_pages) * Hkv * AX_PAGE, static_cast<uint64_t>(D) * es,
+                               AX_PAGE, "k cache")))
+    return rc;
+  if ((rc = make_tmap_bytes_2d(&tmV, vcache, static_cast<uint64_t>(num_pages) * Hkv * D, AX_PAGE * es, D, "v cache"))) return rc;
+  a.q = q;
+  a.q_stride = q_stride;
+  a.gate = static_cast<const bf16*>(gate);
+  a.gate_stride = gate_stride;
+  a.num_pages = num_pages;
+  a.table = page_table;
+  a.pt_stride = pt_stride;
+  a.cu = cu_seqlens;
+  a.seqlens = seqlens;
+  a.B = B;
+  a.T = T;
+  a.hq = Hq;
+  a.hkv = Hkv;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = static_cast<bf16*>(out);
+  a.desc = static_cast<int32_t*>(ws);
+  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + static_cast<size_t>(sm_count()) * 32);
+  a.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid(T * Hkv);
-  if (cache_bf16) {
-    if (D == 256) launch_k(attn_extend_rows_kernel<bf16, 256>, grid, dim3(256), 0, st, a);
-    else launch_k(attn_extend_rows_kernel<bf16, 128>, grid, dim3(256), 0, st, a);
-  } else {
-    if (D == 256) launch_k(attn_extend_rows_kernel<uint8_t, 256>, grid, dim3(256), 0, st, a);
-    else launch_k(attn_extend_rows_kernel<uint8_t, 128>, grid, dim3(256), 0, st, a);
-  }
+  if (cache_bf16)
+    D == 256 ? ax_launch<false, 256>(tmQ, tmK, tmV, a, st) : ax_launch<false, 128>(tmQ, tmK, tmV, a, st);
+  else
+    D == 256 ? ax_launch<true, 256>(tmQ, tmK, tmV, a, st) : ax_launch<true, 128>(tmQ, tmK, tmV, a, st);
   return launch_status("b200_attn_extend");
 }

@@ -46,6 +46,24 @@ int make_tmap_bytes_2d(CUtensorMap* out, const void* base, uint64_t rows, uint64
   return 0;
 }
 
+int make_tmap_bytes_3d(CUtensorMap* out, const void* base, uint64_t row_bytes, uint64_t rows, uint64_t planes,
+                       uint64_t row_stride, uint64_t plane_stride, uint32_t box_rows, uint32_t box_planes, const char* what) {
+  EncodeTiledFn fn = encoder();
+  if (!fn) return fail(B200_E_DRIVER, "%s: cuTensorMapEncodeTiled is not available", what);
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || ((row_stride | plane_stride) & 15) || row_bytes < 128 || rows == 0 || planes == 0)
+    return fail(B200_E_ALIGN, "%s: tensor base / strides must be 16-byte aligned and rows >= 1", what);
+  cuuint64_t dims[3] = {row_bytes, rows, planes};
+  cuuint64_t strides[2] = {row_stride, plane_stride};
+  cuuint32_t box[3] = {128, box_rows, box_planes};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r =
+      fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(B200_E_ARG, "%s: cuTensorMapEncodeTiled failed (%d)", what, static_cast<int>(r));
+  return 0;
+}
+
 int make_tmap_f32_2d(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows,
                      const char* what) {
   EncodeTiledFn fn = encoder();

@@ -48,6 +48,11 @@ inline int launch_status(const char* what) {
 int make_tmap_bytes_2d(CUtensorMap* out, const void* base, uint64_t rows, uint64_t row_bytes, uint32_t box_rows,
                        const char* what);
 
+// 3-D tensor map over bytes [planes][rows][row_bytes] with row and plane strides in bytes (multiples of 16), box
+// [box_planes][box_rows][128 bytes], 128-byte swizzle, zero fill outside.
+int make_tmap_bytes_3d(CUtensorMap* out, const void* base, uint64_t row_bytes, uint64_t rows, uint64_t planes,
+                       uint64_t row_stride, uint64_t plane_stride, uint32_t box_rows, uint32_t box_planes, const char* what);
+
 // 2-D tensor map over a row-major fp32 matrix [rows, cols], box [box_rows, 32 floats], 128-byte swizzle
 int make_tmap_f32_2d(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows,
                      const char* what);
