@@ -88,35 +88,46 @@ struct AxShape {
 __device__ __forceinline__ uint32_t ax_sw128(int row, int chunk) {
   return static_cast<uint32_t>((row >> 3) * 1024 + (row & 7) * 128 + ((chunk ^ (row & 7)) << 4));
 }
-// D += A B with A in tensor memory
+// Shared-memory descriptors of 128-byte-swizzled K-major tiles differ in their low word only (umma_desc_sw128).  The MMAs are
+// issued by one elected lane of a warp whose control flow is uniform, from low words that are a base plus a constant: the
+// operands then stay in uniform registers.  Issued by a lane of a divergent branch with 64-bit descriptors built in place, an
+// MMA took 150 cycles of issue whatever its size; so it takes 64 (N = 128) and 128 (N = 256), the tensor pipe's own time.
+constexpr uint32_t AX_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t ax_desc_lo(uint32_t smem_addr) { return ((smem_addr & 0x3ffffu) >> 4) | (1u << 16); }
+// D += A B, A in tensor memory
 template <bool F8>
-__device__ __forceinline__ void ax_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void ax_mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
   if (F8)
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "{\n.reg .pred p;\n.reg .b64 b;\nsetp.ne.b32 p, %4, 0;\nmov.b64 b, {%2, %5};\n"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], b, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(AX_DESC_HI)
         : "memory");
   else
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "{\n.reg .pred p;\n.reg .b64 b;\nsetp.ne.b32 p, %4, 0;\nmov.b64 b, {%2, %5};\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(AX_DESC_HI)
         : "memory");
 }
+// D += A B, both in shared memory
 template <bool F8>
-__device__ __forceinline__ void ax_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void ax_mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
   if (F8)
-    tc_mma_f8(d, a, b, idesc, accumulate);
+    asm volatile(
+        "{\n.reg .pred p;\n.reg .b64 a, b;\nsetp.ne.b32 p, %4, 0;\nmov.b64 a, {%1, %5};\nmov.b64 b, {%2, %5};\n"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, p;\n}\n" ::"r"(d),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(AX_DESC_HI)
+        : "memory");
   else
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "{\n.reg .pred p;\n.reg .b64 a, b;\nsetp.ne.b32 p, %4, 0;\nmov.b64 a, {%1, %5};\nmov.b64 b, {%2, %5};\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}\n" ::"r"(d),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(AX_DESC_HI)
         : "memory");
 }
 // instruction descriptor: M = 128, N = n, fp32 accumulator, K-major operands
-__device__ __forceinline__ uint32_t ax_idesc(uint32_t a_fmt, uint32_t b_fmt, uint32_t n) {
+__host__ __device__ constexpr uint32_t ax_idesc(uint32_t a_fmt, uint32_t b_fmt, uint32_t n) {
   return (UMMA_C_F32 << 4) | (a_fmt << 7) | (b_fmt << 10) | ((n >> 3) << 17) | ((128u >> 4) << 24);
 }
 __device__ __forceinline__ void ax_tmem_st16(uint32_t taddr, const uint32_t* r) {
@@ -133,14 +144,38 @@ __device__ __forceinline__ float ax_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t ax_e5m2x2(float lo, float hi) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+// two probabilities (f16 pair) to their e5m2 values, in the upper byte of each half: rounded to three significant bits (ties
+// away), which leaves an f16 whose lower byte is zero
+__device__ __forceinline__ uint32_t ax_head(uint32_t h) { return (h + 0x00800080u) & 0xff00ff00u; }
+__device__ __forceinline__ uint32_t ax_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// a probability rounded to three significant bits, which e5m2 holds exactly
-__device__ __forceinline__ float ax_head(float p) {
-  return __uint_as_float((__float_as_uint(p) + 0x00100000u) & 0xffe00000u);
+// e4m3 of the (exact) difference of two f16 pairs, in the low half
+__device__ __forceinline__ uint32_t ax_rest(uint32_t h, uint32_t head) {
+  uint32_t d;
+  uint16_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(h), "r"(head));
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(d));
+  return r;
+}
+__device__ __forceinline__ float ax_max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// (a, b) <- (a, b) * m + c and (a, b) <- (a, b) + (c, d), two fp32 lanes per instruction
+__device__ __forceinline__ void ax_fma2(float& a, float& b, float m, float c) {
+  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%0, %1};\nmov.b64 y, {%2, %2};\nmov.b64 z, {%3, %3};\n"
+      "fma.rn.f32x2 x, x, y, z;\nmov.b64 {%0, %1}, x;\n}\n"
+      : "+f"(a), "+f"(b)
+      : "f"(m), "f"(c));
+}
+__device__ __forceinline__ void ax_add2(float& a, float& b, float c, float d) {
+  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%0, %1};\nmov.b64 y, {%2, %3};\nadd.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}\n"
+      : "+f"(a), "+f"(b)
+      : "f"(c), "f"(d));
 }
 __device__ __forceinline__ void ax_tma_load_3d(void* smem_dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
@@ -209,19 +244,21 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   uint64_t* ifull = vempty + X::NV;       // [AX_ITEMS] item written
   uint64_t* iempty = ifull + AX_ITEMS;    // [AX_ITEMS] all roles are done with it
   uint64_t* sfull = iempty + AX_ITEMS;    // [2] scores complete in TMEM
-  uint64_t* pready = sfull + 2;           // [2] probabilities written (and O rescaled if needed)
-  uint64_t* xch = pready + 2;             // [4] the two warps of a TMEM quadrant published their halves
-  uint64_t* qfull = xch + 4;              // Q tile landed
+  uint64_t* pready = sfull + 2;           // [2 pages][2 halves] probabilities written (and O rescaled if needed)
+  uint64_t* mpub = pready + 4;            // [2 halves][4 quadrants] running maxima published
+  uint64_t* lpub = mpub + 8;              // [4] row sums of both halves published
+  uint64_t* qfull = lpub + 4;             // Q tile landed
   uint64_t* qempty = qfull + 1;           // the item's last score MMA is done
-  uint64_t* pvdone = qempty + 1;          // P . V of a page done
-  uint64_t* ofree = pvdone + 1;           // the accumulator has been read
+  uint64_t* pvdone = qempty + 1;          // [2 halves] P . V of half a page done
+  uint64_t* ofree = pvdone + 2;           // the accumulator has been read
   uint64_t* vtail = ofree + 1;            // [NV] V page with places behind the last key landed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(vtail + X::NV);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_start = reinterpret_cast<int*>(tmem_slot + 2);   // request
   long long* s_off = reinterpret_cast<long long*>(tmem_slot + 4);
   AxItem* items = reinterpret_cast<AxItem*>(smem + X::OFF_ITEM);
-  float* red = reinterpret_cast<float*>(smem + X::OFF_RED);   // [2 pages][2 halves][128 rows]
+  float* s_m = reinterpret_cast<float*>(smem + X::OFF_RED);   // [2 halves][128 rows] running maximum
+  float* s_l = s_m + 256;                                     // [2 halves][128 rows] row sum
   long long* s_scan = reinterpret_cast<long long*>(smem + X::OFF_V);   // prelude only, before any copy is issued
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -241,12 +278,15 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sfull[i], 1);
-      mbar_init(&pready[i], AX_SOFT);
+      mbar_init(&pvdone[i], 1);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&xch[i], 2);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&pready[i], AX_SOFT / 2);
+      mbar_init(&lpub[i], 2);
+    }
+    for (int i = 0; i < 8; ++i) mbar_init(&mpub[i], 1);
     mbar_init(qfull, 1);
     mbar_init(qempty, 1);
-    mbar_init(pvdone, 1);
     mbar_init(ofree, AX_SOFT);
     *abort_flag = 0;
     mbar_fence_init();
@@ -305,7 +345,7 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(FULL_MASK, *tmem_slot, 0);
   const uint32_t TM_O = tmem, TM_S = tmem + 256;   // O: D columns; two score buffers of 128 columns
 
   // items in order; `it` counts them
@@ -530,115 +570,136 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       for (int i = max(0, issued - X::NV); i < issued; ++i) ax_drain(&vfull[i % X::NV], (i / X::NV) & 1);
   } else if (warp == 2) {
     // ---------------- MMA issuer.  The score MMAs run two pages ahead of the P . V MMAs (also into the next item), so the
-    // tensor pipe has a product to do while the softmax warps work on a page ----------------
-    if (lane == 0) {
-      const uint32_t q_base = smem_u32(smem), k_base = smem_u32(smem + X::OFF_K), v_base = smem_u32(smem + X::OFF_V);
-      const uint32_t id_s = ax_idesc(F8 ? 0u : 1u, F8 ? 0u : 1u, 128);
-      const uint32_t id_hi = ax_idesc(1u, F8 ? 0u : 1u, D);     // P: e5m2 or bf16 (both 1); V: e4m3 0 or bf16 1
-      const uint32_t id_lo = ax_idesc(0u, 0u, D);
-      auto get = [&](int it, int& n) -> bool {       // pages of item `it`
-        if (!mbar_wait(&ifull[it % AX_ITEMS], (it / AX_ITEMS) & 1, abort_flag, p.status, ST_WAIT_FULL)) return false;
-        n = items[it % AX_ITEMS].p1 - items[it % AX_ITEMS].p0;
-        return n > 0;
-      };
-      int s_it = 0, s_i = 0, s_n = 0, ts = 0;
-      bool s_more = true, ok = true;
-      auto issue_s = [&]() {
-        if (!s_more) return;
-        if (s_i == s_n) {
-          if (!get(s_it, s_n)) {
-            s_more = false;
-            return;
-          }
-          s_i = 0;
-          if (!mbar_wait(qfull, s_it & 1, abort_flag, p.status, ST_WAIT_FULL)) {
-            s_more = ok = false;
-            return;
-          }
-          ++s_it;
+    // tensor pipe has a product to do while the softmax warps work on a page.  P . V is issued per half page, as its
+    // probabilities arrive ----------------
+    const uint32_t q_lo = ax_desc_lo(smem_u32(smem)), k_lo = ax_desc_lo(smem_u32(smem + X::OFF_K)),
+                   v_lo = ax_desc_lo(smem_u32(smem + X::OFF_V));
+    constexpr uint32_t id_s = ax_idesc(F8 ? 0u : 1u, F8 ? 0u : 1u, 128);
+    constexpr uint32_t id_hi = ax_idesc(1u, F8 ? 0u : 1u, D);     // P: e5m2 or bf16 (both 1); V: e4m3 0 or bf16 1
+    constexpr uint32_t id_lo = ax_idesc(0u, 0u, D);
+    auto get = [&](int it, int& n) -> bool {       // pages of item `it`
+      if (!ax_wait(&ifull[it % AX_ITEMS], (it / AX_ITEMS) & 1, abort_flag, p.status, ST_WAIT_FULL)) return false;
+      n = __shfl_sync(FULL_MASK, items[it % AX_ITEMS].p1 - items[it % AX_ITEMS].p0, 0);
+      return n > 0;
+    };
+    int s_it = 0, s_i = 0, s_n = 0, ts = 0, k_st = 0, k_ph = 0;
+    bool s_more = true, ok = true;
+    auto issue_s = [&]() {
+      if (!s_more) return;
+      if (s_i == s_n) {
+        if (!get(s_it, s_n)) {
+          s_more = false;
+          return;
         }
-        const uint32_t d = TM_S + (ts & 1) * 128;
-        for (int u = 0; u < X::PU; ++u) {
-          const int un = ts * X::PU + u, st = un % X::NK;
-          if (!mbar_wait(&kfull[st], (un / X::NK) & 1, abort_flag, p.status, ST_WAIT_FULL)) {
-            s_more = ok = false;
-            return;
-          }
-          tc_fence_after();
+        s_i = 0;
+        if (!ax_wait(qfull, s_it & 1, abort_flag, p.status, ST_WAIT_FULL)) {
+          s_more = ok = false;
+          return;
+        }
+        ++s_it;
+      }
+      const uint32_t d = TM_S + (ts & 1) * 128;
+#pragma unroll
+      for (int u = 0; u < X::PU; ++u) {
+        if (!ax_wait(&kfull[k_st], k_ph, abort_flag, p.status, ST_WAIT_FULL)) {
+          s_more = ok = false;
+          return;
+        }
+        tc_fence_after();
+        const uint32_t kb = k_lo + k_st * (X::UNIT >> 4);
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < X::UNIT / 16384 * 4; ++kk) {     // 32 bytes of a row per step, four steps per 128-byte block
             const int c = kk >> 2;
-            ax_mma_ss<F8>(d, umma_desc_sw128(q_base + (u * (X::UNIT / 16384) + c) * 16384 + (kk & 3) * 32),
-                          umma_desc_sw128(k_base + st * X::UNIT + c * 16384 + (kk & 3) * 32), id_s, (u | kk) != 0);
+            ax_mma_ss<F8>(d, q_lo + (u * (X::UNIT / 16384) + c) * 1024 + (kk & 3) * 2, kb + c * 1024 + (kk & 3) * 2, id_s,
+                          (u | kk) != 0);
           }
-          tc_commit(&kempty[st]);
-        }
-        tc_commit(&sfull[ts & 1]);
-        ++ts;
-        if (++s_i == s_n) tc_commit(qempty);
-      };
-      issue_s();
-      issue_s();
-      int it = 0, tp = 0, n = 0;
-      while (ok && get(it, n)) {
-        for (int i = 0; ok && i < n; ++i, ++tp) {
-          const int b = tp & 1;
-          ok = mbar_wait(&pready[b], (tp >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
-          if (ok && i == 0 && it > 0) ok = mbar_wait(ofree, (it - 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY);
-          if (!ok) break;
-          const uint32_t pa = TM_S + b * 128;
-          for (int u = 0; u < X::PU; ++u) {
-            const int un = tp * X::PU + u, st = un % X::NV;
-            ok = mbar_wait(&vfull[st], (un / X::NV) & 1, abort_flag, p.status, ST_WAIT_FULL);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t vb = v_base + st * X::UNIT;
-            if (F8) {
-#pragma unroll
-              for (int kk = 0; kk < 4; ++kk)                     // 32 keys a step; the value, then the remainder
-                ax_mma_ts<F8>(TM_O, pa + kk * 8, umma_desc_sw128(vb + kk * 32), id_hi, (i | kk) != 0);
-#pragma unroll
-              for (int kk = 0; kk < 4; ++kk) ax_mma_ts<F8>(TM_O, pa + 32 + kk * 8, umma_desc_sw128(vb + kk * 32), id_lo, 1);
-            } else {
-#pragma unroll
-              for (int kk = 0; kk < 8 / X::PU; ++kk)             // 16 keys a step, four steps per box of 64 keys
-                ax_mma_ts<F8>(TM_O, pa + (u * (8 / X::PU) + kk) * 8, umma_desc_sw128(vb + (kk >> 2) * X::VBOX + (kk & 3) * 32),
-                              id_hi, (i | u | kk) != 0);
-            }
-            tc_commit(&vempty[st]);
+          tc_commit(&kempty[k_st]);
+          if (u == X::PU - 1) {
+            tc_commit(&sfull[ts & 1]);
+            if (s_i == s_n - 1) tc_commit(qempty);
           }
-          if (!ok) break;
-          tc_commit(pvdone);
-          if (i == n - 1) mbar_arrive(&iempty[it % AX_ITEMS]);
-          issue_s();
         }
-        ++it;
+        __syncwarp();
+        if (++k_st == X::NK) {
+          k_st = 0;
+          k_ph ^= 1;
+        }
       }
-      if (*abort_flag) {   // let the MMAs in flight finish before the accumulators are given back
-        tc_commit(qempty);
-        const unsigned long long t0 = globaltimer();
-        while (globaltimer() - t0 < 1000ull * 1000) {
+      ++ts;
+      ++s_i;
+    };
+    issue_s();
+    issue_s();
+    int it = 0, tp = 0, n = 0, v_st = 0, v_ph = 0;
+    while (ok && get(it, n)) {
+      for (int i = 0; ok && i < n; ++i, ++tp) {
+        const int b = tp & 1;
+        const uint32_t pa = TM_S + b * 128;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          if (hf == 0 || X::PU == 2) {
+            ok = ax_wait(&vfull[v_st], v_ph, abort_flag, p.status, ST_WAIT_FULL);
+            if (!ok) break;
+          }
+          ok = ax_wait(&pready[b * 2 + hf], (tp >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
+          if (ok && hf == 0 && i == 0 && it > 0) ok = ax_wait(ofree, (it - 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t vb = v_lo + v_st * (X::UNIT >> 4);
+          if (elect_one()) {
+            if (F8) {     // 32 keys a step; the values, then the remainders
+#pragma unroll
+              for (int kk = 0; kk < 2; ++kk)
+                ax_mma_ts<F8>(TM_O, pa + hf * 64 + kk * 8, vb + (hf * 2 + kk) * 2, id_hi, (i | hf | kk) != 0);
+#pragma unroll
+              for (int kk = 0; kk < 2; ++kk) ax_mma_ts<F8>(TM_O, pa + hf * 64 + 16 + kk * 8, vb + (hf * 2 + kk) * 2, id_lo, 1);
+            } else {      // 16 keys a step; a box holds 64 keys
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                ax_mma_ts<F8>(TM_O, pa + hf * 64 + kk * 8, vb + (X::PU == 2 ? 0 : hf * (X::VBOX >> 4)) + kk * 2, id_hi,
+                              (i | hf | kk) != 0);
+            }
+            if (hf == 1 || X::PU == 2) tc_commit(&vempty[v_st]);
+            tc_commit(&pvdone[hf]);
+            if (hf == 1 && i == n - 1) mbar_arrive(&iempty[it % AX_ITEMS]);
+          }
+          __syncwarp();
+          if ((hf == 1 || X::PU == 2) && ++v_st == X::NV) {
+            v_st = 0;
+            v_ph ^= 1;
+          }
         }
+        if (ok) issue_s();
+      }
+      ++it;
+    }
+    if (*abort_flag) {   // let the MMAs in flight finish before the accumulators are given back
+      const unsigned long long t0 = globaltimer();
+      while (globaltimer() - t0 < 1000ull * 1000) {
       }
     }
   } else {
     // ---------------- softmax: TMEM quadrant q holds rows 32 q ..; of the page's 128 keys warp 4 + q takes 0..63, warp 8 + q
-    // 64..127 ----------------
+    // 64..127.  The running maximum passes from one to the other half page by half page, so neither waits for the other's
+    // exponentials, and P . V of the first half starts without the second.  A half's probabilities go where its scores were ----
     const int q = warp & 3, hf = (warp - AX_SOFT0) >> 2;
     const int row = q * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
     const float sl2 = p.scale_log2;
     const int r_tok = row / p.grp, r_head = row - r_tok * p.grp;
+    uint64_t* m_in = mpub + (hf ^ 1) * 4 + q;
+    uint64_t* m_out = mpub + hf * 4 + q;
     AxItem x;
     int tp = 0;
-    uint32_t xp = 0;                 // phase of this quadrant's exchange barrier
+    uint32_t xp = 0, ep = 0;         // phases of this quadrant: pages, items
     bool ok = true;
     for (int it = 0; ok && item_wait(it, x); ++it) {
       const int n = x.p1 - x.p0;
       const bool active = q * 32 < x.ntok * p.grp;   // warps without a row only take part in the hand-overs
       const bool mine_row = r_tok < x.ntok;
       const int lim = x.pos0 + r_tok;                // last key that this row sees
-      float m = -INFINITY, l = 0.f;
+      float m_own = -INFINITY, l = 0.f;              // the maximum that l is relative to
       const int32_t* tab = p.table + static_cast<size_t>(x.req) * p.pt_stride;
       int id_next = x.p0 < p.pt_stride ? tab[x.p0] : -1;
       for (int i = 0; ok && i < n; ++i, ++tp) {
@@ -649,107 +710,128 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         if (!ok) break;
         if (active) {
           tc_fence_after();
+          const uint32_t sc = TM_S + b * 128 + hf * 64 + lanes;
           uint32_t s[64];
-          tmem_ld32(TM_S + b * 128 + hf * 64 + lanes, *reinterpret_cast<uint32_t(*)[32]>(s));
-          tmem_ld32(TM_S + b * 128 + hf * 64 + 32 + lanes, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
+          tmem_ld32(sc, *reinterpret_cast<uint32_t(*)[32]>(s));
+          tmem_ld32(sc + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
           tmem_ld_wait();
           const bool bad = id < 0 || id >= p.num_pages;
-          if (bad || pg * AX_PAGE + AX_PAGE - 1 > x.pos0) {      // not every row sees the whole page
+          if (bad || pg * AX_PAGE + hf * 64 + 63 > x.pos0) {     // not every row sees all of the half page
             const int see = bad ? -1 : lim - (pg * AX_PAGE + hf * 64);
 #pragma unroll
             for (int j = 0; j < 64; ++j)
               if (j > see) s[j] = 0xff800000u;
           }
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float mx[4];
 #pragma unroll
-          for (int j = 0; j < 64; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(s[j]));
-          const float part = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-          red[(b * 2 + hf) * 128 + row] = part;
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&xch[q]);
-          ok = ax_wait(&xch[q], xp & 1, abort_flag, p.status, ST_WAIT_STATE);
-          ++xp;
-          if (!ok) break;
-          tc_fence_after();
-          const float tm = fmaxf(part, red[(b * 2 + (hf ^ 1)) * 128 + row]);
+          for (int j = 0; j < 4; ++j) mx[j] = __uint_as_float(s[j]);
+#pragma unroll
+          for (int j = 4; j < 60; j += 8) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mx[k] = ax_max3(mx[k], __uint_as_float(s[j + k]), __uint_as_float(s[j + 4 + k]));
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], __uint_as_float(s[60 + k]));
+          const float tm = fmaxf(ax_max3(mx[0], mx[1], mx[2]), mx[3]);
+          // the maximum so far: the other warp's, of this page (second half) or of the page before
+          float m = -INFINITY;
+          if (hf == 1 || xp > 0) {
+            ok = ax_wait(m_in, hf == 1 ? xp & 1 : (xp - 1) & 1, abort_flag, p.status, ST_WAIT_STATE);
+            if (!ok) break;
+            if (hf == 1 || i > 0) m = s_m[(hf ^ 1) * 128 + row];
+          }
           const bool move = (tm - m) * sl2 > AX_TAU;             // m = -inf: any finite maximum; both -inf: NaN, no move
-          if (__any_sync(FULL_MASK, move)) {
-            const float alpha = move ? ax_exp2((m - tm) * sl2) : 1.f;
-            if (move) m = tm;
-            l *= alpha;
-            if (i > 0) {                                         // (the scores of page tp came after P . V of page tp - 2)
-              ok = ax_wait(pvdone, (tp - 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY);
-              if (!ok) break;
-              tc_fence_after();
+          const float m_new = move ? tm : m;
+          s_m[hf * 128 + row] = m_new;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(m_out);
+          ++xp;
+          if (m_new != m_own) {
+            l *= ax_exp2((m_own - m_new) * sl2);
+            m_own = m_new;
+          }
+          if (__any_sync(FULL_MASK, move) && (hf == 1 || i > 0)) {
+            // every P . V before this half page: the scores of page tp came after P . V of page tp - 2
+            const float alpha = move ? ax_exp2((m - m_new) * sl2) : 1.f;
+            if (hf == 0)
+              ok = ax_wait(&pvdone[1], (tp - 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY);
+            else
+              ok = (tp == 0 || ax_wait(&pvdone[0], (tp - 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY)) &&
+                   ax_wait(&pvdone[0], tp & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t v[16];
+              const uint32_t col = TM_O + c * 16 + lanes;
+              tmem_ld16(col, v);
+              tmem_ld_wait();
 #pragma unroll
-              for (int c = 0; c < D / 64; ++c) {                 // this warp's half of the accumulator's columns
-                uint32_t v[32];
-                const uint32_t col = TM_O + hf * (D / 2) + c * 32 + lanes;
-                tmem_ld32(col, v);
-                tmem_ld_wait();
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
-                ax_tmem_st16(col, v);
-                ax_tmem_st16(col + 16, v + 16);
-              }
-              ax_tmem_st_wait();
+              for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
+              ax_tmem_st16(col, v);
             }
           }
-          const float shift = (F8 ? AX_BIAS : 0.f) - (m == -INFINITY ? 0.f : m * sl2);
+          const float shift = (F8 ? AX_BIAS : 0.f) - (m_new == -INFINITY ? 0.f : m_new * sl2);
           float acc[4] = {0.f, 0.f, 0.f, 0.f};
           if (F8) {
             uint32_t hi[16], lo[16];
 #pragma unroll
             for (int w = 0; w < 16; ++w) {
-              float e[4], h[4];
+              float e[4];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                e[j] = ax_exp2(fmaf(__uint_as_float(s[w * 4 + j]), sl2, shift));
-                acc[j] += e[j];
-                h[j] = ax_head(e[j]);
-              }
-              hi[w] = ax_e5m2x2(h[0], h[1]) | (ax_e5m2x2(h[2], h[3]) << 16);
-              lo[w] = e4m3x4(e[0] - h[0], e[1] - h[1], e[2] - h[2], e[3] - h[3]);
+              for (int j = 0; j < 4; ++j) e[j] = __uint_as_float(s[w * 4 + j]);
+              ax_fma2(e[0], e[1], sl2, shift);
+              ax_fma2(e[2], e[3], sl2, shift);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) e[j] = ax_exp2(e[j]);
+              ax_add2(acc[0], acc[1], e[0], e[1]);
+              ax_add2(acc[2], acc[3], e[2], e[3]);
+              const uint32_t f0 = ax_f16x2(e[0], e[1]), f1 = ax_f16x2(e[2], e[3]);
+              const uint32_t h0 = ax_head(f0), h1 = ax_head(f1);
+              hi[w] = __byte_perm(h0, h1, 0x7531);
+              lo[w] = ax_rest(f0, h0) | (ax_rest(f1, h1) << 16);
             }
-            ax_tmem_st16(TM_S + b * 128 + hf * 16 + lanes, hi);
-            ax_tmem_st16(TM_S + b * 128 + 32 + hf * 16 + lanes, lo);
+            ax_tmem_st16(sc, hi);
+            ax_tmem_st16(sc + 16, lo);
           } else {
             uint32_t w16[32];
 #pragma unroll
             for (int w = 0; w < 32; ++w) {
-              const float e0 = ax_exp2(fmaf(__uint_as_float(s[w * 2]), sl2, shift));
-              const float e1 = ax_exp2(fmaf(__uint_as_float(s[w * 2 + 1]), sl2, shift));
-              w16[w] = pack_bf2(e0, e1);
-              acc[w & 1] += bf_lo(w16[w]);        // the row sum takes the rounded values: a common error cancels
-              acc[2 + (w & 1)] += bf_hi(w16[w]);
-            }
-            ax_tmem_st16(TM_S + b * 128 + hf * 32 + lanes, w16);
-            ax_tmem_st16(TM_S + b * 128 + hf * 32 + 16 + lanes, w16 + 16);
+              float e0 = __uint_as_float(s[w * 2]), e1 = __uint_as_float(s[w * 2 + 1]);
+              ax_fma2(e0, e1, sl2, shift);
+              w16[w] = pack_bf2(ax_exp2(e0), ax_exp2(e1));
+              ax_add2(acc[(w & 1) * 2], acc[(w & 1) * 2 + 1], bf_lo(w16[w]), bf_hi(w16[w]));   // the row sum takes the rounded
+            }                                                                                  // values: a common error cancels
+            ax_tmem_st16(sc, w16);
+            ax_tmem_st16(sc + 16, w16 + 16);
           }
           ax_tmem_st_wait();
           l += (acc[0] + acc[1]) + (acc[2] + acc[3]);
           tc_fence_before();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&pready[b]);
+        if (lane == 0) mbar_arrive(&pready[b * 2 + hf]);
       }
       if (!ok) break;
-      // ---- epilogue: the row sum's halves meet, each warp writes its half of the columns of its rows ----
-      // P . V of the page before the last may still be running (its scores came first); its phase must be over before the
-      // last page's can be told from the one before it
-      if (tp >= 2) ok = ax_wait(pvdone, tp & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
-      ok = ok && ax_wait(pvdone, (tp - 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
+      // ---- epilogue: the row sums of the halves meet, each warp writes its half of the columns of its rows.  The last P . V
+      // but one may still be running (its scores came first); its phase must be over before the last one's can be told
+      // from the one before it ----
+      if (tp >= 2) ok = ax_wait(&pvdone[1], tp & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
+      ok = ok && ax_wait(&pvdone[1], (tp - 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
       if (!ok) break;
       if (active) {
         tc_fence_after();
-        red[(((tp - 1) & 1) * 2 + hf) * 128 + row] = l;    // the last page's buffer: everybody has read it
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&xch[q]);
-        ok = ax_wait(&xch[q], xp & 1, abort_flag, p.status, ST_WAIT_STATE);
-        ++xp;
+        if (hf == 0) ok = ax_wait(m_in, (xp - 1) & 1, abort_flag, p.status, ST_WAIT_STATE);
         if (!ok) break;
-        const float total = l + red[(((tp - 1) & 1) * 2 + (hf ^ 1)) * 128 + row];
+        const float m = s_m[128 + row];              // the second half of the last page has the last word
+        if (m_own != m) l *= ax_exp2((m_own - m) * sl2);
+        s_l[hf * 128 + row] = l;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&lpub[q]);
+        ok = ax_wait(&lpub[q], ep & 1, abort_flag, p.status, ST_WAIT_STATE);
+        ++ep;
+        if (!ok) break;
+        const float total = l + s_l[(hf ^ 1) * 128 + row];
         const bool store = mine_row && x.tok0 + r_tok < p.T;
         const long long tok = x.tok0 + r_tok;
         const int col0 = hf * (D / 2);
