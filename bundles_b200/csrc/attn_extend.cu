@@ -249,8 +249,8 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   uint64_t* lpub = mpub + 8;              // [4] row sums of both halves published
   uint64_t* qfull = lpub + 4;             // Q tile landed
   uint64_t* qempty = qfull + 1;           // the item's last score MMA is done
-  uint64_t* pvdone = qempty + 1;          // [2 halves] P . V of half a page done
-  uint64_t* ofree = pvdone + 2;           // the accumulator has been read
+  uint64_t* pvdone = qempty + 1;          // [2 pages][2 halves] P . V of half a page done
+  uint64_t* ofree = pvdone + 4;           // the accumulator has been read
   uint64_t* vtail = ofree + 1;            // [NV] V page with places behind the last key landed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(vtail + X::NV);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -278,9 +278,9 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sfull[i], 1);
-      mbar_init(&pvdone[i], 1);
     }
     for (int i = 0; i < 4; ++i) {
+      mbar_init(&pvdone[i], 1);
       mbar_init(&pready[i], AX_SOFT / 2);
       mbar_init(&lpub[i], 2);
     }
@@ -661,7 +661,7 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                               (i | hf | kk) != 0);
             }
             if (hf == 1 || X::PU == 2) tc_commit(&vempty[v_st]);
-            tc_commit(&pvdone[hf]);
+            tc_commit(&pvdone[b * 2 + hf]);
             if (hf == 1 && i == n - 1) mbar_arrive(&iempty[it % AX_ITEMS]);
           }
           __syncwarp();
@@ -681,8 +681,11 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     }
   } else {
     // ---------------- softmax: TMEM quadrant q holds rows 32 q ..; of the page's 128 keys warp 4 + q takes 0..63, warp 8 + q
-    // 64..127.  The running maximum passes from one to the other half page by half page, so neither waits for the other's
-    // exponentials, and P . V of the first half starts without the second.  A half's probabilities go where its scores were ----
+    // 64..127.  The running maximum passes from one to the other, half page by half page, and hardly ever moves: the first
+    // half's warp has the second's of the page before in hand when the scores arrive, the second half's warp goes on with
+    // its own last one and looks at the end whether the first half moved it (then it does the half page again).  So neither
+    // waits for the other between the scores and the probabilities, and P . V of the first half starts without the second.
+    // A half's probabilities go where its scores were ----------------
     const int q = warp & 3, hf = (warp - AX_SOFT0) >> 2;
     const int row = q * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
@@ -706,80 +709,94 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         const int b = tp & 1, pg = x.p0 + i;
         const int id = id_next;
         if (i + 1 < n) id_next = pg + 1 < p.pt_stride ? tab[pg + 1] : -1;
+        if (!active) {
+          ok = ax_wait(&sfull[b], (tp >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
+          if (ok && lane == 0) mbar_arrive(&pready[b * 2 + hf]);
+          continue;
+        }
+        const bool bad = id < 0 || id >= p.num_pages;
+        const bool edge = bad || pg * AX_PAGE + hf * 64 + 63 > x.pos0;   // not every row sees all of the half page
+        const int see = bad ? -1 : lim - (pg * AX_PAGE + hf * 64);
+        float m = m_own;
+        if (hf == 0 && xp > 0) {
+          ok = ax_wait(m_in, (xp - 1) & 1, abort_flag, p.status, ST_WAIT_STATE);
+          if (!ok) break;
+          if (i > 0) m = s_m[128 + row];
+        }
+        const uint32_t sc = TM_S + b * 128 + hf * 64 + lanes;
         ok = ax_wait(&sfull[b], (tp >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
         if (!ok) break;
-        if (active) {
-          tc_fence_after();
-          const uint32_t sc = TM_S + b * 128 + hf * 64 + lanes;
+        tc_fence_after();
+        bool sure = hf == 0;                         // m is the maximum before this half page
+        float m_new, sum;
+        while (true) {
           uint32_t s[64];
           tmem_ld32(sc, *reinterpret_cast<uint32_t(*)[32]>(s));
           tmem_ld32(sc + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
           tmem_ld_wait();
-          const bool bad = id < 0 || id >= p.num_pages;
-          if (bad || pg * AX_PAGE + hf * 64 + 63 > x.pos0) {     // not every row sees all of the half page
-            const int see = bad ? -1 : lim - (pg * AX_PAGE + hf * 64);
+          if (edge) {
 #pragma unroll
             for (int j = 0; j < 64; ++j)
               if (j > see) s[j] = 0xff800000u;
           }
           float mx[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) mx[j] = __uint_as_float(s[j]);
+          for (int j = 0; j < 4; ++j) mx[j] = ax_max3(__uint_as_float(s[j]), __uint_as_float(s[4 + j]), __uint_as_float(s[8 + j]));
 #pragma unroll
-          for (int j = 4; j < 60; j += 8) {
+          for (int j = 12; j < 60; j += 8) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) mx[k] = ax_max3(mx[k], __uint_as_float(s[j + k]), __uint_as_float(s[j + 4 + k]));
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], __uint_as_float(s[60 + k]));
           const float tm = fmaxf(ax_max3(mx[0], mx[1], mx[2]), mx[3]);
-          // the maximum so far: the other warp's, of this page (second half) or of the page before
-          float m = -INFINITY;
-          if (hf == 1 || xp > 0) {
-            ok = ax_wait(m_in, hf == 1 ? xp & 1 : (xp - 1) & 1, abort_flag, p.status, ST_WAIT_STATE);
-            if (!ok) break;
-            if (hf == 1 || i > 0) m = s_m[(hf ^ 1) * 128 + row];
-          }
-          const bool move = (tm - m) * sl2 > AX_TAU;             // m = -inf: any finite maximum; both -inf: NaN, no move
-          const float m_new = move ? tm : m;
-          s_m[hf * 128 + row] = m_new;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(m_out);
-          ++xp;
-          if (m_new != m_own) {
-            l *= ax_exp2((m_own - m_new) * sl2);
-            m_own = m_new;
-          }
-          if (__any_sync(FULL_MASK, move) && (hf == 1 || i > 0)) {
-            // every P . V before this half page: the scores of page tp came after P . V of page tp - 2
-            const float alpha = move ? ax_exp2((m - m_new) * sl2) : 1.f;
-            if (hf == 0)
-              ok = ax_wait(&pvdone[1], (tp - 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY);
-            else
-              ok = (tp == 0 || ax_wait(&pvdone[0], (tp - 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY)) &&
-                   ax_wait(&pvdone[0], tp & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY);
-            if (!ok) break;
-            tc_fence_after();
-#pragma unroll 1
-            for (int c = 0; c < D / 16; ++c) {
-              uint32_t v[16];
-              const uint32_t col = TM_O + c * 16 + lanes;
-              tmem_ld16(col, v);
-              tmem_ld_wait();
-#pragma unroll
-              for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
-              ax_tmem_st16(col, v);
+          bool move = (tm - m) * sl2 > AX_TAU;       // m = -inf: any finite maximum; both -inf: NaN, no move
+          m_new = m;
+          if (__any_sync(FULL_MASK, move || m != m_own)) {
+            if (!sure) {
+              ok = ax_wait(m_in, xp & 1, abort_flag, p.status, ST_WAIT_STATE);
+              if (!ok) break;
+              sure = true;
+              m = s_m[row];
+              move = (tm - m) * sl2 > AX_TAU;
             }
+            m_new = move ? tm : m;
+            if (m_new != m_own) l *= ax_exp2((m_own - m_new) * sl2);
+            m_own = m_new;
+            if (__any_sync(FULL_MASK, move) && (hf == 1 || i > 0)) {
+              // the P . V just before this half page.  Its barrier's phase before is known to be over (the scores of page tp
+              // came after P . V of page tp - 2) and its next one cannot be (it needs this warp), so the parity is not mistaken
+              const float alpha = move ? ax_exp2((m - m_new) * sl2) : 1.f;
+              ok = hf == 0 ? ax_wait(&pvdone[(b ^ 1) * 2 + 1], ((tp - 1) >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY)
+                           : ax_wait(&pvdone[b * 2], (tp >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY);
+              if (!ok) break;
+              tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < D / 16; ++c) {
+                uint32_t v[16];
+                const uint32_t col = TM_O + c * 16 + lanes;
+                tmem_ld16(col, v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
+                ax_tmem_st16(col, v);
+              }
+            }
+          }
+          if (hf == 0) {
+            s_m[row] = m_new;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(m_out);
           }
           const float shift = (F8 ? AX_BIAS : 0.f) - (m_new == -INFINITY ? 0.f : m_new * sl2);
           float acc[4] = {0.f, 0.f, 0.f, 0.f};
-          if (F8) {
-            uint32_t hi[16], lo[16];
+          uint32_t w[32];
+          if (F8) {     // words 0..15: the values; 16..31: the remainders
 #pragma unroll
-            for (int w = 0; w < 16; ++w) {
+            for (int k = 0; k < 16; ++k) {
               float e[4];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) e[j] = __uint_as_float(s[w * 4 + j]);
+              for (int j = 0; j < 4; ++j) e[j] = __uint_as_float(s[k * 4 + j]);
               ax_fma2(e[0], e[1], sl2, shift);
               ax_fma2(e[2], e[3], sl2, shift);
 #pragma unroll
@@ -788,36 +805,49 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
               ax_add2(acc[2], acc[3], e[2], e[3]);
               const uint32_t f0 = ax_f16x2(e[0], e[1]), f1 = ax_f16x2(e[2], e[3]);
               const uint32_t h0 = ax_head(f0), h1 = ax_head(f1);
-              hi[w] = __byte_perm(h0, h1, 0x7531);
-              lo[w] = ax_rest(f0, h0) | (ax_rest(f1, h1) << 16);
+              w[k] = __byte_perm(h0, h1, 0x7531);
+              w[16 + k] = ax_rest(f0, h0) | (ax_rest(f1, h1) << 16);
             }
-            ax_tmem_st16(sc, hi);
-            ax_tmem_st16(sc + 16, lo);
           } else {
-            uint32_t w16[32];
 #pragma unroll
-            for (int w = 0; w < 32; ++w) {
-              float e0 = __uint_as_float(s[w * 2]), e1 = __uint_as_float(s[w * 2 + 1]);
+            for (int k = 0; k < 32; ++k) {
+              float e0 = __uint_as_float(s[k * 2]), e1 = __uint_as_float(s[k * 2 + 1]);
               ax_fma2(e0, e1, sl2, shift);
-              w16[w] = pack_bf2(ax_exp2(e0), ax_exp2(e1));
-              ax_add2(acc[(w & 1) * 2], acc[(w & 1) * 2 + 1], bf_lo(w16[w]), bf_hi(w16[w]));   // the row sum takes the rounded
-            }                                                                                  // values: a common error cancels
-            ax_tmem_st16(sc, w16);
-            ax_tmem_st16(sc + 16, w16 + 16);
+              w[k] = pack_bf2(ax_exp2(e0), ax_exp2(e1));
+              ax_add2(acc[(k & 1) * 2], acc[(k & 1) * 2 + 1], bf_lo(w[k]), bf_hi(w[k]));   // the row sum takes the rounded
+            }                                                                              // values: a common error cancels
           }
-          ax_tmem_st_wait();
-          l += (acc[0] + acc[1]) + (acc[2] + acc[3]);
-          tc_fence_before();
+          sum = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+          if (!sure) {
+            ok = ax_wait(m_in, xp & 1, abort_flag, p.status, ST_WAIT_STATE);
+            if (!ok) break;
+            sure = true;
+            const float now = s_m[row];
+            if (__any_sync(FULL_MASK, now != m)) {
+              m = now;
+              continue;
+            }
+          }
+          ax_tmem_st16(sc, w);
+          ax_tmem_st16(sc + 16, w + 16);
+          break;
         }
+        if (!ok) break;
+        if (hf == 1) {
+          s_m[128 + row] = m_new;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(m_out);
+        }
+        ++xp;
+        l += sum;
+        ax_tmem_st_wait();
+        tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&pready[b * 2 + hf]);
       }
       if (!ok) break;
-      // ---- epilogue: the row sums of the halves meet, each warp writes its half of the columns of its rows.  The last P . V
-      // but one may still be running (its scores came first); its phase must be over before the last one's can be told
-      // from the one before it ----
-      if (tp >= 2) ok = ax_wait(&pvdone[1], tp & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
-      ok = ok && ax_wait(&pvdone[1], (tp - 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
+      // ---- epilogue: the row sums of the halves meet, each warp writes its half of the columns of its rows ----
+      ok = ax_wait(&pvdone[((tp - 1) & 1) * 2 + 1], ((tp - 1) >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
       if (!ok) break;
       if (active) {
         tc_fence_after();
