@@ -244,21 +244,21 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   uint64_t* ifull = vempty + X::NV;       // [AX_ITEMS] item written
   uint64_t* iempty = ifull + AX_ITEMS;    // [AX_ITEMS] all roles are done with it
   uint64_t* sfull = iempty + AX_ITEMS;    // [2] scores complete in TMEM
-  uint64_t* pready = sfull + 2;           // [2 pages][2 halves] probabilities written (and O rescaled if needed)
-  uint64_t* mpub = pready + 4;            // [2 halves][4 quadrants] running maxima published
-  uint64_t* lpub = mpub + 8;              // [4] row sums of both halves published
+  uint64_t* pready = sfull + 2;           // [2 pages][4 quarters] probabilities written (and O rescaled if needed)
+  uint64_t* mpub = pready + 8;            // [2 page parities][4 quadrants] running maximum published
+  uint64_t* lpub = mpub + 8;              // [4] both warps' row sums published, the last P . V done
   uint64_t* qfull = lpub + 4;             // Q tile landed
   uint64_t* qempty = qfull + 1;           // the item's last score MMA is done
-  uint64_t* pvdone = qempty + 1;          // [2 pages][2 halves] P . V of half a page done
-  uint64_t* ofree = pvdone + 4;           // the accumulator has been read
+  uint64_t* pvdone = qempty + 1;          // [2 pages] P . V of a page done
+  uint64_t* ofree = pvdone + 2;           // the accumulator has been read
   uint64_t* vtail = ofree + 1;            // [NV] V page with places behind the last key landed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(vtail + X::NV);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_start = reinterpret_cast<int*>(tmem_slot + 2);   // request
   long long* s_off = reinterpret_cast<long long*>(tmem_slot + 4);
   AxItem* items = reinterpret_cast<AxItem*>(smem + X::OFF_ITEM);
-  float* s_m = reinterpret_cast<float*>(smem + X::OFF_RED);   // [2 halves][128 rows] running maximum
-  float* s_l = s_m + 256;                                     // [2 halves][128 rows] row sum
+  float* s_m = reinterpret_cast<float*>(smem + X::OFF_RED);   // [2 page parities][128 rows] running maximum
+  float* s_l = s_m + 256;                                     // [2 page parities][128 rows] row sum
   long long* s_scan = reinterpret_cast<long long*>(smem + X::OFF_V);   // prelude only, before any copy is issued
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -278,13 +278,13 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sfull[i], 1);
-    }
-    for (int i = 0; i < 4; ++i) {
       mbar_init(&pvdone[i], 1);
-      mbar_init(&pready[i], AX_SOFT / 2);
-      mbar_init(&lpub[i], 2);
     }
-    for (int i = 0; i < 8; ++i) mbar_init(&mpub[i], 1);
+    for (int i = 0; i < 4; ++i) mbar_init(&lpub[i], 2);
+    for (int i = 0; i < 8; ++i) {
+      mbar_init(&pready[i], AX_SOFT / 2);
+      mbar_init(&mpub[i], 1);
+    }
     mbar_init(qfull, 1);
     mbar_init(qempty, 1);
     mbar_init(ofree, AX_SOFT);
@@ -570,8 +570,8 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       for (int i = max(0, issued - X::NV); i < issued; ++i) ax_drain(&vfull[i % X::NV], (i / X::NV) & 1);
   } else if (warp == 2) {
     // ---------------- MMA issuer.  The score MMAs run two pages ahead of the P . V MMAs (also into the next item), so the
-    // tensor pipe has a product to do while the softmax warps work on a page.  P . V is issued per half page, as its
-    // probabilities arrive ----------------
+    // tensor pipe has a product to do while the softmax warps work on a page.  P . V is issued per quarter of a page, as
+    // its probabilities arrive ----------------
     const uint32_t q_lo = ax_desc_lo(smem_u32(smem)), k_lo = ax_desc_lo(smem_u32(smem + X::OFF_K)),
                    v_lo = ax_desc_lo(smem_u32(smem + X::OFF_V));
     constexpr uint32_t id_s = ax_idesc(F8 ? 0u : 1u, F8 ? 0u : 1u, 128);
@@ -637,35 +637,35 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         const int b = tp & 1;
         const uint32_t pa = TM_S + b * 128;
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          if (hf == 0 || X::PU == 2) {
+        for (int c = 0; c < 4; ++c) {          // 32 keys each
+          if (c == 0 || (X::PU == 2 && c == 2)) {
             ok = ax_wait(&vfull[v_st], v_ph, abort_flag, p.status, ST_WAIT_FULL);
             if (!ok) break;
           }
-          ok = ax_wait(&pready[b * 2 + hf], (tp >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
-          if (ok && hf == 0 && i == 0 && it > 0) ok = ax_wait(ofree, (it - 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY);
+          ok = ax_wait(&pready[b * 4 + c], (tp >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
+          if (ok && c == 0 && i == 0 && it > 0) ok = ax_wait(ofree, (it - 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY);
           if (!ok) break;
           tc_fence_after();
           const uint32_t vb = v_lo + v_st * (X::UNIT >> 4);
+          const bool unit_end = c == 3 || (X::PU == 2 && c == 1);
           if (elect_one()) {
-            if (F8) {     // 32 keys a step; the values, then the remainders
-#pragma unroll
-              for (int kk = 0; kk < 2; ++kk)
-                ax_mma_ts<F8>(TM_O, pa + hf * 64 + kk * 8, vb + (hf * 2 + kk) * 2, id_hi, (i | hf | kk) != 0);
-#pragma unroll
-              for (int kk = 0; kk < 2; ++kk) ax_mma_ts<F8>(TM_O, pa + hf * 64 + 16 + kk * 8, vb + (hf * 2 + kk) * 2, id_lo, 1);
+            if (F8) {     // the values, then the remainders
+              ax_mma_ts<F8>(TM_O, pa + c * 32, vb + c * 2, id_hi, (i | c) != 0);
+              ax_mma_ts<F8>(TM_O, pa + c * 32 + 8, vb + c * 2, id_lo, 1);
             } else {      // 16 keys a step; a box holds 64 keys
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk)
-                ax_mma_ts<F8>(TM_O, pa + hf * 64 + kk * 8, vb + (X::PU == 2 ? 0 : hf * (X::VBOX >> 4)) + kk * 2, id_hi,
-                              (i | hf | kk) != 0);
+              for (int kk = 0; kk < 2; ++kk)
+                ax_mma_ts<F8>(TM_O, pa + c * 32 + kk * 8,
+                              vb + (X::PU == 2 ? 0 : (c >> 1) * (X::VBOX >> 4)) + ((c & 1) * 2 + kk) * 2, id_hi, (i | c | kk) != 0);
             }
-            if (hf == 1 || X::PU == 2) tc_commit(&vempty[v_st]);
-            tc_commit(&pvdone[b * 2 + hf]);
-            if (hf == 1 && i == n - 1) mbar_arrive(&iempty[it % AX_ITEMS]);
+            if (unit_end) tc_commit(&vempty[v_st]);
+            if (c == 3) {
+              tc_commit(&pvdone[b]);
+              if (i == n - 1) mbar_arrive(&iempty[it % AX_ITEMS]);
+            }
           }
           __syncwarp();
-          if ((hf == 1 || X::PU == 2) && ++v_st == X::NV) {
+          if (unit_end && ++v_st == X::NV) {
             v_st = 0;
             v_ph ^= 1;
           }
@@ -680,196 +680,188 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       }
     }
   } else {
-    // ---------------- softmax: TMEM quadrant q holds rows 32 q ..; of the page's 128 keys warp 4 + q takes 0..63, warp 8 + q
-    // 64..127.  The running maximum passes from one to the other, half page by half page, and hardly ever moves: the first
-    // half's warp has the second's of the page before in hand when the scores arrive, the second half's warp goes on with
-    // its own last one and looks at the end whether the first half moved it (then it does the half page again).  So neither
-    // waits for the other between the scores and the probabilities, and P . V of the first half starts without the second.
-    // A half's probabilities go where its scores were ----------------
-    const int q = warp & 3, hf = (warp - AX_SOFT0) >> 2;
+    // ---------------- softmax: TMEM quadrant q holds rows 32 q .., a lane owns a row.  Warp 4 + q takes the even pages and
+    // warp 8 + q the odd ones (they share a scheduler: while one reads scores and looks for their maximum the other keeps
+    // the exponential unit busy), and the running maximum passes between them ahead of the exponentials.  The probabilities
+    // of 32 keys go where their scores were, and to the MMA issuer quarter by quarter ----------------
+    const int q = warp & 3, e = (warp - AX_SOFT0) >> 2;
     const int row = q * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
+    const uint32_t sc = TM_S + e * 128 + lanes;
     const float sl2 = p.scale_log2;
     const int r_tok = row / p.grp, r_head = row - r_tok * p.grp;
-    uint64_t* m_in = mpub + (hf ^ 1) * 4 + q;
-    uint64_t* m_out = mpub + hf * 4 + q;
     AxItem x;
-    int tp = 0;
-    uint32_t xp = 0, ep = 0;         // phases of this quadrant: pages, items
+    int tp0 = 0;                     // pages of the items before
+    uint32_t pub = 0;                // maxima published by the other warp of the quadrant
+    uint32_t ep = 0;                 // items of this quadrant
     bool ok = true;
     for (int it = 0; ok && item_wait(it, x); ++it) {
       const int n = x.p1 - x.p0;
       const bool active = q * 32 < x.ntok * p.grp;   // warps without a row only take part in the hand-overs
-      const bool mine_row = r_tok < x.ntok;
       const int lim = x.pos0 + r_tok;                // last key that this row sees
-      float m_own = -INFINITY, l = 0.f;              // the maximum that l is relative to
       const int32_t* tab = p.table + static_cast<size_t>(x.req) * p.pt_stride;
-      int id_next = x.p0 < p.pt_stride ? tab[x.p0] : -1;
-      for (int i = 0; ok && i < n; ++i, ++tp) {
-        const int b = tp & 1, pg = x.p0 + i;
-        const int id = id_next;
-        if (i + 1 < n) id_next = pg + 1 < p.pt_stride ? tab[pg + 1] : -1;
+      float m_own = -INFINITY, l = 0.f;              // the maximum that l is relative to
+      uint32_t bad = 0;                              // missing pages among 32
+      for (int i = (tp0 & 1) ^ e; ok && i < n; i += 2) {
+        const int tp = tp0 + i, pg = x.p0 + i;
         if (!active) {
-          ok = ax_wait(&sfull[b], (tp >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
-          if (ok && lane == 0) mbar_arrive(&pready[b * 2 + hf]);
+          ok = ax_wait(&sfull[e], (tp >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
+          if (ok && lane < 4) mbar_arrive(&pready[e * 4 + lane]);
           continue;
         }
-        const bool bad = id < 0 || id >= p.num_pages;
-        const bool edge = bad || pg * AX_PAGE + hf * 64 + 63 > x.pos0;   // not every row sees all of the half page
-        const int see = bad ? -1 : lim - (pg * AX_PAGE + hf * 64);
-        float m = m_own;
-        if (hf == 0 && xp > 0) {
-          ok = ax_wait(m_in, (xp - 1) & 1, abort_flag, p.status, ST_WAIT_STATE);
-          if (!ok) break;
-          if (i > 0) m = s_m[128 + row];
+        if ((i & 31) < 2) {
+          const int j = pg - (i & 31) + lane;
+          const int id = j < x.p1 && j < p.pt_stride ? tab[j] : -1;
+          bad = __ballot_sync(FULL_MASK, j < x.p1 && (id < 0 || id >= p.num_pages));
         }
-        const uint32_t sc = TM_S + b * 128 + hf * 64 + lanes;
-        ok = ax_wait(&sfull[b], (tp >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
+        const bool gone = (bad >> (i & 31)) & 1;
+        const bool edge = gone || pg * AX_PAGE + AX_PAGE - 1 > x.pos0;   // not every row sees all of the page
+        const int see = gone ? -1 : lim - pg * AX_PAGE;
+        ok = ax_wait(&sfull[e], (tp >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
         if (!ok) break;
         tc_fence_after();
-        bool sure = hf == 0;                         // m is the maximum before this half page
-        float m_new, sum;
-        while (true) {
-          uint32_t s[64];
-          tmem_ld32(sc, *reinterpret_cast<uint32_t(*)[32]>(s));
-          tmem_ld32(sc + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
-          tmem_ld_wait();
-          if (edge) {
+        if (edge) {                                  // masked in place, so that the two passes below need not ask
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c) {
+            uint32_t v[16];
+            tmem_ld16(sc + c * 16, v);
+            tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 64; ++j)
-              if (j > see) s[j] = 0xff800000u;
+            for (int j = 0; j < 16; ++j)
+              if (c * 16 + j > see) v[j] = 0xff800000u;
+            ax_tmem_st16(sc + c * 16, v);
           }
-          float mx[4];
+          ax_tmem_st_wait();
+        }
+        // the loops over a row's scores stay rolled: unrolled, a page's code overran the instruction cache, and the warps
+        // waited for instructions a quarter of the time
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+        for (int g = 0; g < 2; ++g) {
+          uint32_t s[64];
+          tmem_ld32(sc + g * 64, *reinterpret_cast<uint32_t(*)[32]>(s));
+          tmem_ld32(sc + g * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
+          tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 4; ++j) mx[j] = ax_max3(__uint_as_float(s[j]), __uint_as_float(s[4 + j]), __uint_as_float(s[8 + j]));
-#pragma unroll
-          for (int j = 12; j < 60; j += 8) {
+          for (int j = 0; j < 64; j += 8) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) mx[k] = ax_max3(mx[k], __uint_as_float(s[j + k]), __uint_as_float(s[j + 4 + k]));
           }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], __uint_as_float(s[60 + k]));
-          const float tm = fmaxf(ax_max3(mx[0], mx[1], mx[2]), mx[3]);
-          bool move = (tm - m) * sl2 > AX_TAU;       // m = -inf: any finite maximum; both -inf: NaN, no move
-          m_new = m;
-          if (__any_sync(FULL_MASK, move || m != m_own)) {
-            if (!sure) {
-              ok = ax_wait(m_in, xp & 1, abort_flag, p.status, ST_WAIT_STATE);
-              if (!ok) break;
-              sure = true;
-              m = s_m[row];
-              move = (tm - m) * sl2 > AX_TAU;
-            }
-            m_new = move ? tm : m;
-            if (m_new != m_own) l *= ax_exp2((m_own - m_new) * sl2);
-            m_own = m_new;
-            if (__any_sync(FULL_MASK, move) && (hf == 1 || i > 0)) {
-              // the P . V just before this half page.  Its barrier's phase before is known to be over (the scores of page tp
-              // came after P . V of page tp - 2) and its next one cannot be (it needs this warp), so the parity is not mistaken
-              const float alpha = move ? ax_exp2((m - m_new) * sl2) : 1.f;
-              ok = hf == 0 ? ax_wait(&pvdone[(b ^ 1) * 2 + 1], ((tp - 1) >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY)
-                           : ax_wait(&pvdone[b * 2], (tp >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY);
-              if (!ok) break;
-              tc_fence_after();
+        }
+        const float tm = fmaxf(ax_max3(mx[0], mx[1], mx[2]), mx[3]);
+        // the maximum so far, of the page before
+        float m = -INFINITY;
+        if (i > 0) {
+          ok = ax_wait(&mpub[(e ^ 1) * 4 + q], (pub + ((i + 1) >> 1) - 1) & 1, abort_flag, p.status, ST_WAIT_STATE);
+          if (!ok) break;
+          m = s_m[(e ^ 1) * 128 + row];
+        }
+        const bool move = (tm - m) * sl2 > AX_TAU;   // m = -inf: any finite maximum; both -inf: NaN, no move
+        const float m_new = move ? tm : m;
+        s_m[e * 128 + row] = m_new;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&mpub[e * 4 + q]);
+        if (__any_sync(FULL_MASK, m_new != m_own)) {
+          if (m_new != m_own) l *= ax_exp2((m_own - m_new) * sl2);
+          m_own = m_new;
+          if (i > 0 && __any_sync(FULL_MASK, move)) {
+            // P . V of the page before.  Its barrier's phase before is known to be over (the scores of page tp came after
+            // P . V of page tp - 2) and its next one cannot be (it needs this page), so the parity is not mistaken
+            const float alpha = move ? ax_exp2((m - m_new) * sl2) : 1.f;
+            ok = ax_wait(&pvdone[e ^ 1], ((tp - 1) >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY);
+            if (!ok) break;
+            tc_fence_after();
 #pragma unroll 1
-              for (int c = 0; c < D / 16; ++c) {
-                uint32_t v[16];
-                const uint32_t col = TM_O + c * 16 + lanes;
-                tmem_ld16(col, v);
-                tmem_ld_wait();
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t v[16];
+              const uint32_t col = TM_O + c * 16 + lanes;
+              tmem_ld16(col, v);
+              tmem_ld_wait();
 #pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
-                ax_tmem_st16(col, v);
-              }
+              for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
+              ax_tmem_st16(col, v);
             }
           }
-          if (hf == 0) {
-            s_m[row] = m_new;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(m_out);
-          }
-          const float shift = (F8 ? AX_BIAS : 0.f) - (m_new == -INFINITY ? 0.f : m_new * sl2);
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-          uint32_t w[32];
-          if (F8) {     // words 0..15: the values; 16..31: the remainders
+        }
+        const float shift = (F8 ? AX_BIAS : 0.f) - (m_new == -INFINITY ? 0.f : m_new * sl2);
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[32];
+          tmem_ld32(sc + c * 32, v);
+          tmem_ld_wait();
+          uint32_t w[16];
+          if (F8) {     // words 0..7: the values; 8..15: the remainders
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              float e[4];
+            for (int k = 0; k < 8; ++k) {
+              float f[4];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) e[j] = __uint_as_float(s[k * 4 + j]);
-              ax_fma2(e[0], e[1], sl2, shift);
-              ax_fma2(e[2], e[3], sl2, shift);
+              for (int j = 0; j < 4; ++j) f[j] = __uint_as_float(v[k * 4 + j]);
+              ax_fma2(f[0], f[1], sl2, shift);
+              ax_fma2(f[2], f[3], sl2, shift);
 #pragma unroll
-              for (int j = 0; j < 4; ++j) e[j] = ax_exp2(e[j]);
-              ax_add2(acc[0], acc[1], e[0], e[1]);
-              ax_add2(acc[2], acc[3], e[2], e[3]);
-              const uint32_t f0 = ax_f16x2(e[0], e[1]), f1 = ax_f16x2(e[2], e[3]);
+              for (int j = 0; j < 4; ++j) f[j] = ax_exp2(f[j]);
+              ax_add2(acc[0], acc[1], f[0], f[1]);
+              ax_add2(acc[2], acc[3], f[2], f[3]);
+              const uint32_t f0 = ax_f16x2(f[0], f[1]), f1 = ax_f16x2(f[2], f[3]);
               const uint32_t h0 = ax_head(f0), h1 = ax_head(f1);
               w[k] = __byte_perm(h0, h1, 0x7531);
-              w[16 + k] = ax_rest(f0, h0) | (ax_rest(f1, h1) << 16);
+              w[8 + k] = ax_rest(f0, h0) | (ax_rest(f1, h1) << 16);
             }
           } else {
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              float e0 = __uint_as_float(s[k * 2]), e1 = __uint_as_float(s[k * 2 + 1]);
-              ax_fma2(e0, e1, sl2, shift);
-              w[k] = pack_bf2(ax_exp2(e0), ax_exp2(e1));
+            for (int k = 0; k < 16; ++k) {
+              float f0 = __uint_as_float(v[k * 2]), f1 = __uint_as_float(v[k * 2 + 1]);
+              ax_fma2(f0, f1, sl2, shift);
+              w[k] = pack_bf2(ax_exp2(f0), ax_exp2(f1));
               ax_add2(acc[(k & 1) * 2], acc[(k & 1) * 2 + 1], bf_lo(w[k]), bf_hi(w[k]));   // the row sum takes the rounded
             }                                                                              // values: a common error cancels
           }
-          sum = (acc[0] + acc[1]) + (acc[2] + acc[3]);
-          if (!sure) {
-            ok = ax_wait(m_in, xp & 1, abort_flag, p.status, ST_WAIT_STATE);
-            if (!ok) break;
-            sure = true;
-            const float now = s_m[row];
-            if (__any_sync(FULL_MASK, now != m)) {
-              m = now;
-              continue;
-            }
-          }
-          ax_tmem_st16(sc, w);
-          ax_tmem_st16(sc + 16, w + 16);
-          break;
-        }
-        if (!ok) break;
-        if (hf == 1) {
-          s_m[128 + row] = m_new;
+          ax_tmem_st16(sc + c * 32, w);
+          ax_tmem_st_wait();
+          tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(m_out);
+          if (lane == 0) mbar_arrive(&pready[e * 4 + c]);
         }
-        ++xp;
-        l += sum;
-        ax_tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&pready[b * 2 + hf]);
+        l += (acc[0] + acc[1]) + (acc[2] + acc[3]);
       }
       if (!ok) break;
-      // ---- epilogue: the row sums of the halves meet, each warp writes its half of the columns of its rows ----
-      ok = ax_wait(&pvdone[((tp - 1) & 1) * 2 + 1], ((tp - 1) >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
+      // ---- epilogue: the row sums of the two warps meet, each writes half of the columns of its rows ----
+      const int last = tp0 + n - 1;                  // the last page; its warp knows when its P . V is done
+      const bool mine = (last & 1) == e;
+      const long long tok = x.tok0 + r_tok;
+      const bool store = r_tok < x.ntok && tok < p.T;
+      const int col0 = e * (D / 2);
+      uint4 gv[D / 16];
+      if (p.gate && store && x.slot < 0) {           // requested before the last P . V is waited for
+        const uint4* g = reinterpret_cast<const uint4*>(p.gate + tok * p.gate_stride + (x.head * p.grp + r_head) * D + col0);
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) gv[j] = g[j];
+      }
+      if (mine) ok = ax_wait(&pvdone[e], (last >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
       if (!ok) break;
       if (active) {
-        tc_fence_after();
-        if (hf == 0) ok = ax_wait(m_in, (xp - 1) & 1, abort_flag, p.status, ST_WAIT_STATE);
-        if (!ok) break;
-        const float m = s_m[128 + row];              // the second half of the last page has the last word
-        if (m_own != m) l *= ax_exp2((m_own - m) * sl2);
-        s_l[hf * 128 + row] = l;
+        pub += (n + ((tp0 & 1) ^ e)) >> 1;           // the other warp's pages: the larger half if it had the first
+        float m = m_own;
+        if (!mine) {
+          ok = ax_wait(&mpub[(e ^ 1) * 4 + q], (pub - 1) & 1, abort_flag, p.status, ST_WAIT_STATE);
+          if (!ok) break;
+          m = s_m[(e ^ 1) * 128 + row];
+          if (m_own != m) l *= ax_exp2((m_own - m) * sl2);
+        }
+        s_l[e * 128 + row] = l;
+        tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&lpub[q]);
         ok = ax_wait(&lpub[q], ep & 1, abort_flag, p.status, ST_WAIT_STATE);
         ++ep;
         if (!ok) break;
-        const float total = l + s_l[(hf ^ 1) * 128 + row];
-        const bool store = mine_row && x.tok0 + r_tok < p.T;
-        const long long tok = x.tok0 + r_tok;
-        const int col0 = hf * (D / 2);
+        tc_fence_after();
+        const float total = l + s_l[(e ^ 1) * 128 + row];
         const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
         bf16* o = p.out + (tok * p.hq + x.head * p.grp + r_head) * D + col0;
-        const bf16* g = p.gate ? p.gate + tok * p.gate_stride + (x.head * p.grp + r_head) * D + col0 : nullptr;
         float* po = p.part + (static_cast<size_t>(max(x.slot, 0)) * p.rows + row) * D + col0;
-#pragma unroll 1
+#pragma unroll
         for (int c = 0; c < D / 64; ++c) {
           uint32_t v[32];
           tmem_ld32(TM_O + col0 + c * 32 + lanes, v);
@@ -883,14 +875,13 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             for (int j = 0; j < 4; ++j) {
               float f[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(v[j * 8 + e]) * inv;
-              if (g) {
-                const uint4 gv = reinterpret_cast<const uint4*>(g + c * 32)[j];
-                const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w};
+              for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(v[j * 8 + k]) * inv;
+              if (p.gate) {
+                const uint32_t gw[4] = {gv[c * 4 + j].x, gv[c * 4 + j].y, gv[c * 4 + j].z, gv[c * 4 + j].w};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  f[e * 2] = __fdividef(f[e * 2], 1.f + __expf(-bf_lo(gw[e])));
-                  f[e * 2 + 1] = __fdividef(f[e * 2 + 1], 1.f + __expf(-bf_hi(gw[e])));
+                for (int k = 0; k < 4; ++k) {
+                  f[k * 2] = __fdividef(f[k * 2], 1.f + __expf(-bf_lo(gw[k])));
+                  f[k * 2 + 1] = __fdividef(f[k * 2 + 1], 1.f + __expf(-bf_hi(gw[k])));
                 }
               }
               reinterpret_cast<uint4*>(o + c * 32)[j] =
@@ -899,13 +890,14 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           }
           __syncwarp();
         }
-        if (x.slot >= 0 && store && hf == 0) {
+        if (x.slot >= 0 && store && e == 0) {
           float* ml = p.part + static_cast<size_t>(2 * grid) * p.rows * D + static_cast<size_t>(x.slot) * 2 * p.rows;
           ml[row] = m * sl2;
           ml[p.rows + row] = total;
         }
         tc_fence_before();
       }
+      tp0 += n;
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(ofree);
