@@ -77,8 +77,9 @@ struct AxShape {
   static constexpr int OFF_K = QB;
   static constexpr int OFF_V = OFF_K + NK * UNIT;
   static constexpr int OFF_BAR = OFF_V + NV * UNIT;
-  static constexpr int OFF_ITEM = OFF_BAR + 512;   // at most 60 barriers and 24 bytes
+  static constexpr int OFF_ITEM = OFF_BAR + 640;   // barriers and 24 bytes
   static constexpr int OFF_RED = OFF_ITEM + AX_ITEMS * 32;
+  static_assert((2 * NK + 3 * NV + 2 * AX_ITEMS + 30) * 8 + 24 <= 640, "room for the barriers");
   static constexpr int SMEM = OFF_RED + 2 * 2 * 128 * 4;
   static_assert(SMEM <= 232448, "shared memory of a CTA");
   static constexpr int VBOX = D * 128;                 // one V box: D rows of 128 bytes
@@ -215,9 +216,14 @@ __device__ __forceinline__ long long ax_cost_all(int n, int ctx, int tpt) {
   return ax_cost((n - 1) / tpt, ctx, tpt) + AX_OVH + ax_pages(ctx + n);
 }
 
-// Waits of a whole warp: every lane polls, and all give up together.
-__device__ __forceinline__ bool ax_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+// Waits of a whole warp: every lane polls, and all give up together.  The wait proper stays out of line: most barriers are
+// complete when they are asked for, and the MMA issuer's own instructions have to fit between its MMAs.
+__device__ __noinline__ bool ax_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
   return __all_sync(FULL_MASK, mbar_wait(bar, parity, abort_flag, status, code));
+}
+__device__ __forceinline__ bool ax_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  if (__all_sync(FULL_MASK, mbar_try(bar, parity))) return true;
+  return ax_wait_slow(bar, parity, abort_flag, status, code);
 }
 // After an abandoned wait: gives a copy or a commit that is still in flight a bounded time.
 __device__ __forceinline__ void ax_drain(uint64_t* bar, uint32_t parity) {
@@ -250,8 +256,9 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   uint64_t* qfull = lpub + 4;             // Q tile landed
   uint64_t* qempty = qfull + 1;           // the item's last score MMA is done
   uint64_t* pvdone = qempty + 1;          // [2 pages] P . V of a page done
-  uint64_t* ofree = pvdone + 2;           // the accumulator has been read
-  uint64_t* vtail = ofree + 1;            // [NV] V page with places behind the last key landed
+  uint64_t* ofree = pvdone + 2;           // [AX_ITEMS] the item's accumulator has been read (by ring place: a warp without rows
+                                          // may be some items ahead, and must not arrive twice in one phase)
+  uint64_t* vtail = ofree + AX_ITEMS;            // [NV] V page with places behind the last key landed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(vtail + X::NV);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_start = reinterpret_cast<int*>(tmem_slot + 2);   // request
@@ -275,6 +282,7 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     for (int i = 0; i < AX_ITEMS; ++i) {
       mbar_init(&ifull[i], 1);
       mbar_init(&iempty[i], 3 + AX_SOFT);   // K, V, MMA, softmax warps
+      mbar_init(&ofree[i], AX_SOFT);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sfull[i], 1);
@@ -287,7 +295,6 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     }
     mbar_init(qfull, 1);
     mbar_init(qempty, 1);
-    mbar_init(ofree, AX_SOFT);
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmQ);
@@ -643,7 +650,7 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             if (!ok) break;
           }
           ok = ax_wait(&pready[b * 4 + c], (tp >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
-          if (ok && c == 0 && i == 0 && it > 0) ok = ax_wait(ofree, (it - 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY);
+          if (ok && c == 0 && i == 0 && it > 0) ok = ax_wait(&ofree[(it - 1) % AX_ITEMS], ((it - 1) / AX_ITEMS) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY);
           if (!ok) break;
           tc_fence_after();
           const uint32_t vb = v_lo + v_st * (X::UNIT >> 4);
@@ -900,7 +907,7 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       tp0 += n;
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(ofree);
+        mbar_arrive(&ofree[it % AX_ITEMS]);
         mbar_arrive(&iempty[it % AX_ITEMS]);
       }
     }
