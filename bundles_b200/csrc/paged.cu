@@ -167,26 +167,118 @@ __global__ void __launch_bounds__(PP_THREADS) page_plan_kernel(const PlanArgs p)
   }
 }
 
-// One CTA per (token, kv head).
+// The append copies K rows as they are and turns V rows into columns of the dim-major pages.  A CTA takes the tokens that fill
+// 128 bytes of a page's V row (KA_TOK) and 64 dims of one kv head.  The tokens are cut into pieces that share one aligned
+// 16-byte chunk of a page (a new piece starts where the slots do not follow on, and at every chunk); eight neighbouring
+// lanes take neighbouring pieces of the same dims, so whole pages are written in full 128-byte lines.  A piece that is not
+// a whole chunk (a lone decoded token) is written element by element.  V passes through shared memory in 4-byte words
+// whose place is rotated by the piece, so that the eight lanes read different banks.
+// Bound: HBM for prompts; the two dependent loads (slot, row) and the launch for a decode step.
+constexpr int KA_DIMS = 64, KA_THREADS = 128;
+
 template <typename E>
-__global__ void __launch_bounds__(256) kv_append_rows_kernel(const E* __restrict__ k, const E* __restrict__ v,
-                                                             long long k_stride, long long v_stride, int hkv, int dim,
-                                                             E* __restrict__ kc, E* __restrict__ vc, int num_pages,
-                                                             const int64_t* __restrict__ slots, int32_t* status) {
+__global__ void __launch_bounds__(KA_THREADS) kv_append_kernel(const E* __restrict__ k, const E* __restrict__ v,
+                                                               long long k_stride, long long v_stride, int T, int hkv, int dim,
+                                                               E* __restrict__ kc, E* __restrict__ vc, int num_pages,
+                                                               const int64_t* __restrict__ slots, int32_t* status) {
+  constexpr int ES = sizeof(E), KA_TOK = 128 / ES, G = 16 / ES;   // tokens of the tile, of a chunk
+  constexpr int ROW_W = KA_DIMS * ES / 4, ROW_Q = KA_DIMS * ES / 16;   // words and 16-byte quarters of a token's slice
+  constexpr int PER_W = 4 / ES;                                    // dims of a word
+  __shared__ long long s_slot[KA_TOK];
+  __shared__ int s_start[KA_TOK + 1];
+  __shared__ int s_cnt[4];
+  __shared__ __align__(16) uint32_t s_v[KA_TOK * ROW_W];
   pdl_wait();
   pdl_launch();
-  const int t = blockIdx.x / hkv, h = blockIdx.x % hkv, d = threadIdx.x;
-  const long long slot = slots[t];
-  if (slot < 0) return;
-  const long long page = slot / PG_TOKENS;
-  const int o = static_cast<int>(slot % PG_TOKENS);
-  if (page >= num_pages) {
-    if (d == 0) flag(status, B200_ST_BAD_PAGE);
-    return;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int slices = dim / KA_DIMS;
+  const int d0 = (blockIdx.x % slices) * KA_DIMS, h = (blockIdx.x / slices) % hkv;
+  const long long t0 = static_cast<long long>(blockIdx.x / slices / hkv) * KA_TOK;
+  const int n = static_cast<int>(min(static_cast<long long>(KA_TOK), T - t0));
+  long long slot = -1;
+  if (tid < n) {
+    slot = slots[t0 + tid];
+    if (slot >= static_cast<long long>(num_pages) * PG_TOKENS) {
+      flag(status, B200_ST_BAD_PAGE);
+      slot = -1;
+    }
+    if (slot < 0) slot = -1;
   }
-  const size_t ph = static_cast<size_t>(page) * hkv + h;
-  kc[(ph * PG_TOKENS + o) * dim + d] = k[t * k_stride + h * dim + d];
-  vc[(ph * dim + d) * PG_TOKENS + o] = v[t * v_stride + h * dim + d];
+  if (tid < KA_TOK) s_slot[tid] = slot;
+  // both tiles are requested before the slots are looked at
+  constexpr int LD = KA_TOK * ROW_Q / KA_THREADS;
+  uint4 kr[LD], vr[LD];
+#pragma unroll
+  for (int i = 0; i < LD; ++i) {
+    const int t = (tid + i * KA_THREADS) / ROW_Q, c = (tid + i * KA_THREADS) % ROW_Q;
+    if (t < n) {
+      kr[i] = *reinterpret_cast<const uint4*>(k + (t0 + t) * k_stride + static_cast<long long>(h) * dim + d0 + c * G);
+      vr[i] = *reinterpret_cast<const uint4*>(v + (t0 + t) * v_stride + static_cast<long long>(h) * dim + d0 + c * G);
+    }
+  }
+  __syncthreads();
+  const bool start = tid < n && (tid == 0 || slot != s_slot[tid - 1] + 1 || slot % G == 0 || slot < 0);
+  const unsigned ball = __ballot_sync(FULL_MASK, start);
+  if (lane == 0) s_cnt[warp] = __popc(ball);
+#pragma unroll
+  for (int i = 0; i < LD; ++i) {
+    const int t = (tid + i * KA_THREADS) / ROW_Q, c = (tid + i * KA_THREADS) % ROW_Q;
+    if (t < n) {
+      const long long sl = s_slot[t];
+      if (sl >= 0) *reinterpret_cast<uint4*>(kc + ((sl / PG_TOKENS * hkv + h) * PG_TOKENS + sl % PG_TOKENS) * dim + d0 + c * G) = kr[i];
+      // a token's words are rotated by 4 for every chunk's worth of tokens
+      uint32_t* row = s_v + t * ROW_W;
+      const int rot = (t / G) * 4;
+      *reinterpret_cast<uint4*>(row + ((c * 4 + rot) & (ROW_W - 1))) = vr[i];
+    }
+  }
+  __syncthreads();
+  int before = 0, pieces = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < warp) before += s_cnt[w];
+    pieces += s_cnt[w];
+  }
+  if (start) s_start[before + __popc(ball & ((1u << lane) - 1))] = tid;
+  if (tid == 0) s_start[pieces] = n;
+  __syncthreads();
+  // items: 8 pieces x the words of a slice, pieces fastest
+  const int items = (pieces + 7) / 8 * 8 * ROW_W;
+  for (int it = tid; it < items; it += KA_THREADS) {
+    const int pc = it / (8 * ROW_W) * 8 + (it & 7), wd = (it >> 3) % ROW_W;
+    if (pc >= pieces) continue;
+    const int a = s_start[pc], cnt = s_start[pc + 1] - a;
+    const long long sl = s_slot[a];
+    if (sl < 0) continue;
+    E* dst = vc + ((sl / PG_TOKENS * hkv + h) * dim + d0 + wd * PER_W) * PG_TOKENS + sl % PG_TOKENS;
+    auto word = [&](int t) -> uint32_t { return s_v[t * ROW_W + ((wd + (t / G) * 4) & (ROW_W - 1))]; };
+    if (cnt == G) {
+      uint32_t x[G];
+#pragma unroll
+      for (int j = 0; j < G; ++j) x[j] = word(a + j);
+#pragma unroll
+      for (int e = 0; e < PER_W; ++e) {   // dim e of the word: its elements of the G tokens, side by side
+        uint32_t y[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (ES == 1) {
+            const uint32_t lo = __byte_perm(x[q * 4], x[q * 4 + 1], e | ((4 + e) << 4));
+            const uint32_t hi = __byte_perm(x[q * 4 + 2], x[q * 4 + 3], e | ((4 + e) << 4));
+            y[q] = __byte_perm(lo, hi, 0x5410);
+          } else {
+            y[q] = __byte_perm(x[q * 2], x[q * 2 + 1], e ? 0x7632 : 0x5410);
+          }
+        }
+        *reinterpret_cast<uint4*>(dst + e * PG_TOKENS) = make_uint4(y[0], y[1], y[2], y[3]);
+      }
+    } else {
+      for (int j = 0; j < cnt; ++j) {
+        const uint32_t x = word(a + j);
+#pragma unroll
+        for (int e = 0; e < PER_W; ++e) dst[e * PG_TOKENS + j] = static_cast<E>(x >> (e * 8 * ES));
+      }
+    }
+  }
 }
 
 }  // namespace b200
@@ -232,14 +324,15 @@ extern "C" int b200_kv_append(const void* k, const void* v, long long k_stride, 
     return fail(B200_E_ALIGN, "b200_kv_append: tensors and token strides must be 16-byte aligned");
   if (T == 0) return 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (static_cast<long long>(T) * Hkv > 0x7fffffffll) return fail(B200_E_ARG, "b200_kv_append: T * Hkv must stay below 2^31");
+  const long long tok = cache_bf16 ? 64 : 128, grid = (T + tok - 1) / tok * Hkv * (D / KA_DIMS);
+  if (grid > 0x7fffffffll) return fail(B200_E_ARG, "b200_kv_append: too many tokens (T=%d)", T);
   if (cache_bf16)
-    launch_k(kv_append_rows_kernel<uint16_t>, dim3(T * Hkv), dim3(D), 0, st, static_cast<const uint16_t*>(k),
-             static_cast<const uint16_t*>(v), k_stride, v_stride, Hkv, D, static_cast<uint16_t*>(kcache),
-             static_cast<uint16_t*>(vcache), num_pages, slots, status);
+    launch_k(kv_append_kernel<uint16_t>, dim3(static_cast<unsigned>(grid)), dim3(KA_THREADS), 0, st,
+             static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), k_stride, v_stride, T, Hkv, D,
+             static_cast<uint16_t*>(kcache), static_cast<uint16_t*>(vcache), num_pages, slots, status);
   else
-    launch_k(kv_append_rows_kernel<uint8_t>, dim3(T * Hkv), dim3(D), 0, st, static_cast<const uint8_t*>(k),
-             static_cast<const uint8_t*>(v), k_stride, v_stride, Hkv, D, static_cast<uint8_t*>(kcache),
-             static_cast<uint8_t*>(vcache), num_pages, slots, status);
+    launch_k(kv_append_kernel<uint8_t>, dim3(static_cast<unsigned>(grid)), dim3(KA_THREADS), 0, st,
+             static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v), k_stride, v_stride, T, Hkv, D,
+             static_cast<uint8_t*>(kcache), static_cast<uint8_t*>(vcache), num_pages, slots, status);
   return launch_status("b200_kv_append");
 }

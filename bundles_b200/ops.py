@@ -412,29 +412,28 @@ class PagePlan(NamedTuple):
     n_left: torch.Tensor        # int32 [1]: pages left on the free list
 
 
-def _launch(what, fn, device, *args):
-    """Calls `fn` on `device`'s current stream, whichever device is current."""
-    if device.index == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+_raw_stream = torch._C._cuda_getCurrentRawStream     # the current stream of a device, without a Stream object around it
+
+
+def _launch(what, fn, index, *args):
+    """Calls `fn` on the current stream of device `index`, whichever device is current."""
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        check(rc, what)
 
 
-def _together(what, device, *tensors):
+def _together(what, index, *tensors):
     for t in tensors:
-        if t is not None and t.device != device:
-            raise B200Error(f"{what}: tensors on {device} and {t.device}")
+        if t is not None and t.get_device() != index:
+            raise B200Error(f"{what}: all tensors must be on one device (cuda:{index} and {t.device})")
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
-
-
-def _need_status(what, status, device):
-    if status is not None:
-        _need(status, torch.int32, "status")
-        _together(what, device, status)
 
 
 def _token_rows(t, dtype, name, heads=None, dim=None):
@@ -474,7 +473,7 @@ def page_plan(ctx_lens, new_lens, page_table, num_pages, max_tokens, free_pages=
     _need(ctx_lens, torch.int32, "ctx_lens", 1)
     _need(new_lens, torch.int32, "new_lens", 1)
     _need(page_table, torch.int32, "page_table", 2)
-    B, dev, T = ctx_lens.shape[0], ctx_lens.device, int(max_tokens)
+    B, dev, T = ctx_lens.shape[0], ctx_lens.get_device(), int(max_tokens)
     if new_lens.shape[0] != B or page_table.shape[0] != B:
         raise B200Error("page_plan: ctx_lens, new_lens and page_table must have one entry per request")
     if free_pages is not None:
@@ -484,14 +483,15 @@ def page_plan(ctx_lens, new_lens, page_table, num_pages, max_tokens, free_pages=
         _need(n_free, torch.int32, "n_free")
         if n_free.numel() != 1:
             raise B200Error("page_plan: n_free must have one element")
-    _together("page_plan", dev, new_lens, page_table, free_pages, n_free)
-    _need_status("page_plan", status, dev)
+    if status is not None:
+        _need(status, torch.int32, "status")
+    _together("page_plan", dev, new_lens, page_table, free_pages, n_free, status)
     if out is None:
         if T <= 0 or B == 0:
             raise B200Error(f"page_plan: need at least one request and one row (B={B} max_tokens={T})")
-        i32, i64 = dict(dtype=torch.int32, device=dev), dict(dtype=torch.int64, device=dev)
-        out = PagePlan(torch.empty(B + 1, **i32), torch.empty(B, **i32), torch.empty(T, **i64), torch.empty(T, **i64),
-                       torch.empty(1, **i32))
+        new, device = ctx_lens.new_empty, ctx_lens.device
+        out = PagePlan(new(B + 1), new(B), torch.empty(T, dtype=torch.int64, device=device),
+                       torch.empty(T, dtype=torch.int64, device=device), new(1))
     else:
         for t, dt, n in ((out.cu_seqlens, torch.int32, B + 1), (out.seqlens, torch.int32, B), (out.positions, torch.int64, T),
                          (out.slots, torch.int64, T), (out.n_left, torch.int32, 1)):
@@ -517,11 +517,13 @@ def kv_append(k, v, kcache, vcache, slots, status=None):
     T = k.shape[0]
     if v.shape[0] != T or slots.shape[0] != T:
         raise B200Error("kv_append: k, v and slots must have one row per token")
-    _together("kv_append", kcache.device, k, v, vcache, slots)
-    _need_status("kv_append", status, kcache.device)
+    if status is not None:
+        _need(status, torch.int32, "status")
+    dev = kcache.get_device()
+    _together("kv_append", dev, k, v, vcache, slots, status)
     if T == 0:
         return
-    _launch("b200_kv_append", _lib.lib().b200_kv_append, kcache.device, k.data_ptr(), v.data_ptr(), ks, vs, T, hkv, D,
+    _launch("b200_kv_append", _lib.lib().b200_kv_append, dev, k.data_ptr(), v.data_ptr(), ks, vs, T, hkv, D,
             1 if dt == torch.bfloat16 else 0, kcache.data_ptr(), vcache.data_ptr(), P, slots.data_ptr(), _ptr(status))
 
 
@@ -542,13 +544,14 @@ def attn_extend(q, gate, kcache, vcache, page_table, cu_seqlens, seqlens, scale=
     _need(page_table, torch.int32, "page_table", 2)
     _need(cu_seqlens, torch.int32, "cu_seqlens", 1)
     _need(seqlens, torch.int32, "seqlens", 1)
-    B, dev = seqlens.shape[0], q.device
+    B, dev = seqlens.shape[0], q.get_device()
     if cu_seqlens.shape[0] != B + 1 or page_table.shape[0] != B:
         raise B200Error("attn_extend: page_table [B, W], cu_seqlens [B + 1] and seqlens [B] do not fit together")
-    _together("attn_extend", dev, gate, kcache, vcache, page_table, cu_seqlens, seqlens, out, ws)
-    _need_status("attn_extend", status, dev)
+    if status is not None:
+        _need(status, torch.int32, "status")
+    _together("attn_extend", dev, gate, kcache, vcache, page_table, cu_seqlens, seqlens, out, ws, status)
     if out is None:
-        out = torch.empty(T, hq * D, dtype=torch.bfloat16, device=dev)
+        out = torch.empty(T, hq * D, dtype=torch.bfloat16, device=q.device)
     else:
         _need(out, torch.bfloat16, "out", 2)
         if tuple(out.shape) != (T, hq * D):
@@ -556,7 +559,7 @@ def attn_extend(q, gate, kcache, vcache, page_table, cu_seqlens, seqlens, scale=
     if T == 0:
         return out
     if ws is None:
-        ws = attn_extend_workspace(T, hq, hkv, D, dev)
+        ws = attn_extend_workspace(T, hq, hkv, D, q.device)
     else:
         _need(ws, torch.uint8, "ws", 1)
     _launch("b200_attn_extend", _lib.lib().b200_attn_extend, dev, q.data_ptr(), qs, _ptr(gate), gs, kcache.data_ptr(),
