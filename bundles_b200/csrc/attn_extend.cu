@@ -52,7 +52,7 @@ struct AxArgs {
   float scale_log2;
   bf16* out;
   int32_t* desc;                 // [grid][8]: tiles to merge
-  float* part;                   // [2 * grid][rows][D] unnormalised, then [2 * grid][2][rows]: maximum, row sum
+  float* part;                   // [2 * grid][D / 4][rows][4] unnormalised, then [2 * grid][2][rows]: maximum, row sum
   int rows;                      // tpt * grp
   int32_t* status;
 };
@@ -79,11 +79,12 @@ struct AxShape {
   static constexpr int OFF_BAR = OFF_V + NV * UNIT;
   static constexpr int OFF_ITEM = OFF_BAR + 640;   // barriers and 24 bytes
   static constexpr int OFF_RED = OFF_ITEM + AX_ITEMS * 32;
-  static_assert((2 * NK + 3 * NV + 2 * AX_ITEMS + 30) * 8 + 24 <= 640, "room for the barriers");
   static constexpr int SMEM = OFF_RED + 2 * 2 * 128 * 4;
   static_assert(SMEM <= 232448, "shared memory of a CTA");
   static constexpr int VBOX = D * 128;                 // one V box: D rows of 128 bytes
   static constexpr int NVB = ES;                       // boxes per V page
+  static constexpr int NS = D == 128 ? 3 : 2;          // score buffers: what the accumulator leaves of 512 columns
+  static_assert((2 * NK + 3 * NV + 3 * AX_ITEMS + 6 * NS + 14) * 8 + 24 <= 640, "room for the barriers");
 };
 
 __device__ __forceinline__ uint32_t ax_sw128(int row, int chunk) {
@@ -178,6 +179,27 @@ __device__ __forceinline__ void ax_add2(float& a, float& b, float c, float d) {
       : "+f"(a), "+f"(b)
       : "f"(c), "f"(d));
 }
+// 8 x 8 transposition of 16-byte pieces among 8 neighbouring lanes: piece k of lane b becomes piece b of lane k
+__device__ __forceinline__ void ax_exchange8(uint4 (&x)[8], int lane) {
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) {
+    const bool up = (lane & o) != 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if ((k & o) == 0) {
+        const uint4 send = up ? x[k] : x[k | o];
+        uint4 got;
+        got.x = __shfl_xor_sync(FULL_MASK, send.x, o);
+        got.y = __shfl_xor_sync(FULL_MASK, send.y, o);
+        got.z = __shfl_xor_sync(FULL_MASK, send.z, o);
+        got.w = __shfl_xor_sync(FULL_MASK, send.w, o);
+        if (up)
+          x[k] = got;
+        else
+          x[k | o] = got;
+      }
+  }
+}
 __device__ __forceinline__ void ax_tma_load_3d(void* smem_dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
@@ -185,23 +207,28 @@ __device__ __forceinline__ void ax_tma_load_3d(void* smem_dst, const CUtensorMap
       : "memory");
 }
 
-// sum over i < m of floor((a + i s) / d); a, s >= 0, d > 0 (Euclid's descent on (d, s))
-__device__ __forceinline__ long long ax_floor_sum(long long m, long long d, long long s, long long a) {
+// sum over i < m of floor((a + i s) / d); s <= 128, d <= 128, m <= 2^24 (Euclid's descent on (d, s); every divide in 32 bits)
+__device__ __forceinline__ long long ax_floor_sum(uint32_t m, uint32_t d, uint32_t s, uint32_t a) {
   long long r = 0;
   while (m > 0) {
-    r += m * (a / d);
+    r += static_cast<long long>(m) * (a / d);
     a %= d;
-    r += m * (m - 1) / 2 * (s / d);
+    r += static_cast<long long>(m) * (m - 1) / 2 * (s / d);
     s %= d;
-    const long long y = s * m + a;
+    const uint32_t y = s * m + a;
     if (y < d) break;
     m = y / d;
     a = y % d;
-    const long long t = d;
+    const uint32_t t = d;
     d = s;
     s = t;
   }
   return r;
+}
+// x / y, in 32 bits where both fit
+__device__ __forceinline__ long long ax_div(long long x, long long y) {
+  if (((x | y) >> 32) == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(y);
+  return x / y;
 }
 // pages that a tile reads whose last token sees keys 0 .. end - 1
 __device__ __forceinline__ int ax_pages(int end) { return end <= 0 ? 0 : (end + AX_PAGE - 1) / AX_PAGE; }
@@ -209,7 +236,7 @@ __device__ __forceinline__ int ax_pages(int end) { return end <= 0 ? 0 : (end + 
 __device__ __forceinline__ long long ax_cost(int k, int ctx, int tpt) {
   const int skip = ctx < 0 ? min(k, -ctx / tpt) : 0;   // tiles whose last token sees nothing
   return static_cast<long long>(k) * AX_OVH +
-         ax_floor_sum(k - skip, AX_PAGE, tpt, static_cast<long long>(ctx) + static_cast<long long>(skip + 1) * tpt + AX_PAGE - 1);
+         ax_floor_sum(k - skip, AX_PAGE, tpt, static_cast<uint32_t>(ctx + (skip + 1) * tpt + AX_PAGE - 1));
 }
 __device__ __forceinline__ long long ax_cost_all(int n, int ctx, int tpt) {
   if (n <= 0) return 0;
@@ -224,6 +251,15 @@ __device__ __noinline__ bool ax_wait_slow(uint64_t* bar, uint32_t parity, volati
 __device__ __forceinline__ bool ax_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
   if (__all_sync(FULL_MASK, mbar_try(bar, parity))) return true;
   return ax_wait_slow(bar, parity, abort_flag, status, code);
+}
+__device__ __forceinline__ bool ax_test(uint64_t* bar, uint32_t parity) {   // without waiting
+  uint32_t ok;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 // After an abandoned wait: gives a copy or a commit that is still in flight a bounded time.
 __device__ __forceinline__ void ax_drain(uint64_t* bar, uint32_t parity) {
@@ -249,14 +285,14 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   uint64_t* vempty = vfull + X::NV;       // [NV]
   uint64_t* ifull = vempty + X::NV;       // [AX_ITEMS] item written
   uint64_t* iempty = ifull + AX_ITEMS;    // [AX_ITEMS] all roles are done with it
-  uint64_t* sfull = iempty + AX_ITEMS;    // [2] scores complete in TMEM
-  uint64_t* pready = sfull + 2;           // [2 pages][4 quarters] probabilities written (and O rescaled if needed)
-  uint64_t* mpub = pready + 8;            // [2 page parities][4 quadrants] running maximum published
+  uint64_t* sfull = iempty + AX_ITEMS;    // [NS] scores complete in TMEM
+  uint64_t* pready = sfull + X::NS;       // [NS][4 quarters] probabilities written (and O rescaled if needed)
+  uint64_t* mpub = pready + 4 * X::NS;            // [2 page parities][4 quadrants] running maximum published
   uint64_t* lpub = mpub + 8;              // [4] both warps' row sums published, the last P . V done
   uint64_t* qfull = lpub + 4;             // Q tile landed
   uint64_t* qempty = qfull + 1;           // the item's last score MMA is done
-  uint64_t* pvdone = qempty + 1;          // [2 pages] P . V of a page done
-  uint64_t* ofree = pvdone + 2;           // [AX_ITEMS] the item's accumulator has been read (by ring place: a warp without rows
+  uint64_t* pvdone = qempty + 1;          // [NS] P . V of a page done
+  uint64_t* ofree = pvdone + X::NS;           // [AX_ITEMS] the item's accumulator has been read (by ring place: a warp without rows
                                           // may be some items ahead, and must not arrive twice in one phase)
   uint64_t* vtail = ofree + AX_ITEMS;            // [NV] V page with places behind the last key landed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(vtail + X::NV);
@@ -284,15 +320,13 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       mbar_init(&iempty[i], 3 + AX_SOFT);   // K, V, MMA, softmax warps
       mbar_init(&ofree[i], AX_SOFT);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < X::NS; ++i) {
       mbar_init(&sfull[i], 1);
       mbar_init(&pvdone[i], 1);
     }
+    for (int i = 0; i < 4 * X::NS; ++i) mbar_init(&pready[i], AX_SOFT / 2);
     for (int i = 0; i < 4; ++i) mbar_init(&lpub[i], 2);
-    for (int i = 0; i < 8; ++i) {
-      mbar_init(&pready[i], AX_SOFT / 2);
-      mbar_init(&mpub[i], 1);
-    }
+    for (int i = 0; i < 8; ++i) mbar_init(&mpub[i], 1);
     mbar_init(qfull, 1);
     mbar_init(qempty, 1);
     *abort_flag = 0;
@@ -329,11 +363,19 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     C += v;
   }
   const long long U = C * p.hkv;
-  const long long n_want = (U + AX_MIN_UNITS - 1) / AX_MIN_UNITS;
-  const int n_eff = n_want > grid ? grid : static_cast<int>(n_want);
-  const long long u0 = cta < n_eff ? cta * U / n_eff : U, u1 = cta < n_eff ? (cta + 1) * U / n_eff : U;
+  // n_eff ranges: the first `more` of them have `each` + 1 units, the others `each`
+  const int n_eff = U >= static_cast<long long>(grid) * AX_MIN_UNITS ? grid : static_cast<int>((U + AX_MIN_UNITS - 1) / AX_MIN_UNITS);
+  const long long each = n_eff ? ax_div(U, n_eff) : 0;
+  const int more = static_cast<int>(U - each * n_eff);
+  auto bound = [&](int c) -> long long { return c * each + min(c, more); };
+  auto range_of = [&](long long u) -> int {   // the range that holds unit u
+    const long long lo = more * (each + 1);
+    return static_cast<int>(u < lo ? ax_div(u, each + 1) : more + ax_div(u - lo, each));
+  };
+  const long long u0 = cta < n_eff ? bound(cta) : U, u1 = cta < n_eff ? bound(cta + 1) : U;
+  const int head0 = u0 < u1 ? static_cast<int>(ax_div(u0, C)) : 0;
   if (u0 < u1) {
-    const long long v0 = u0 % C;
+    const long long v0 = u0 - head0 * C;
     if (v0 >= before && v0 < before + mine) {
       long long at = before;
       for (int b = b0; b < b1; ++b) {
@@ -353,7 +395,7 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(FULL_MASK, *tmem_slot, 0);
-  const uint32_t TM_O = tmem, TM_S = tmem + 256;   // O: D columns; two score buffers of 128 columns
+  const uint32_t TM_O = tmem, TM_S = tmem + 512 - X::NS * 128;   // O: D columns; NS score buffers of 128
 
   // items in order; `it` counts them
   auto item_wait = [&](int it, AxItem& x) -> bool {
@@ -369,47 +411,73 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   if (warp == 3) {
     // ---------------- scheduler: walks the tiles of this CTA's range.  The same warp clears, in the copy of the last V page
     // of an item, the places behind the last key that its tile sees: they may hold anything, and a zero probability
-    // times a NaN would spoil the row.  Such a page lands on a barrier of its own and counts as full once it is cleared.
-    // An item is cleared before its place in the ring is waited for, so neither duty holds up the other ----------------
-    int it = 0, cl = 0, pages = 0;   // items written, items cleared, pages of the cleared ones
-    uint32_t tails = 0;              // per stage: phase of its tail barrier
+    // times a NaN would spoil the row.  Such a page lands on a barrier of its own and counts as full once it is cleared; it is
+    // tended whenever it lands, also while a place in the item ring is waited for ----------------
+    int it = 0, cl = 0, cu = 0, pages = 0;   // items written; items cleared, units of the next one; pages of the cleared ones
+    uint32_t tails = 0;                      // per stage: phase of its tail barrier
     bool ok = true, described = false;
-    auto clear = [&]() -> bool {
+    auto tend = [&]() -> bool {              // clears the next such unit if it has landed
+      if (cl == it) return false;
       const AxItem x = items[cl % AX_ITEMS];
       const int last = x.pos0 + x.ntok - (x.p1 - 1) * AX_PAGE;
-      ++cl;
-      pages += x.p1 - x.p0;
-      if (last >= AX_PAGE) return true;
-      for (int u = 0; u < X::PU; ++u) {
-        const int un = (pages - 1) * X::PU + u, st = un % X::NV;
-        if (!ax_wait(&vtail[st], (tails >> st) & 1, abort_flag, p.status, ST_WAIT_FULL)) return false;
+      if (last < AX_PAGE) {
+        const int st = ((pages + x.p1 - x.p0 - 1) * X::PU + cu) % X::NV;
+        if (!__all_sync(FULL_MASK, ax_test(&vtail[st], (tails >> st) & 1))) return false;
         tails ^= 1u << st;
+#pragma unroll 1
         for (int c = 0; c < X::UNIT / X::VBOX; ++c) {
-          const int vb = min(128, max(0, last * X::ES - (u * (X::UNIT / X::VBOX) + c) * 128));   // valid bytes of a row of the box
+          const int vb = min(128, max(0, last * X::ES - (cu * (X::UNIT / X::VBOX) + c) * 128));   // valid bytes of a row of the box
           uint8_t* box = smem + X::OFF_V + st * X::UNIT + c * X::VBOX;
-          for (int d = lane; d < D; d += 32)
-            for (int ch = vb >> 4; ch < 8; ++ch) {
-              uint32_t* w = reinterpret_cast<uint32_t*>(box + ax_sw128(d, ch));
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int keep = vb - ch * 16 - e * 4;         // bytes of this word that are valid
-                if (keep <= 0)
-                  w[e] = 0;
-                else if (keep < 4)
-                  w[e] &= 0xffffffffu >> (32 - keep * 8);
-              }
+#pragma unroll 1
+          for (int ch = vb >> 4; ch < 8; ++ch) {
+            uint4 keep;                      // bytes of the chunk that are valid
+            keep.x = vb - ch * 16 >= 4 ? ~0u : vb - ch * 16 <= 0 ? 0u : 0xffffffffu >> (32 - (vb - ch * 16) * 8);
+            keep.y = vb - ch * 16 >= 8 ? ~0u : vb - ch * 16 <= 4 ? 0u : 0xffffffffu >> (32 - (vb - ch * 16 - 4) * 8);
+            keep.z = vb - ch * 16 >= 12 ? ~0u : vb - ch * 16 <= 8 ? 0u : 0xffffffffu >> (32 - (vb - ch * 16 - 8) * 8);
+            keep.w = vb - ch * 16 >= 16 ? ~0u : vb - ch * 16 <= 12 ? 0u : 0xffffffffu >> (32 - (vb - ch * 16 - 12) * 8);
+#pragma unroll 4
+            for (int d = lane; d < D; d += 32) {
+              uint4* w = reinterpret_cast<uint4*>(box + ax_sw128(d, ch));
+              uint4 v = *w;
+              v.x &= keep.x;
+              v.y &= keep.y;
+              v.z &= keep.z;
+              v.w &= keep.w;
+              *w = v;
             }
+          }
         }
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(&vfull[st]);
+        if (++cu < X::PU) return true;
       }
+      cu = 0;
+      pages += x.p1 - x.p0;
+      ++cl;
       return true;
+    };
+    // tends the tails until `done` holds
+    auto until = [&](auto done) -> bool {
+      const unsigned long long t0 = globaltimer();
+      while (true) {
+        if (tend()) continue;
+        if (done()) return true;
+        __nanosleep(32);
+        const bool late = globaltimer() - t0 > g_wait_budget_ns;
+        if (__any_sync(FULL_MASK, *abort_flag || late)) {
+          if (late) {
+            *abort_flag = 1;
+            if (p.status) atomicCAS(p.status, 0, ST_WAIT_EMPTY);
+          }
+          return false;
+        }
+      }
     };
     auto push = [&](const AxItem& x) -> bool {
       const int s = it % AX_ITEMS;
-      if (it >= AX_ITEMS && !clear()) return false;
-      if (!ax_wait(&iempty[s], ((it / AX_ITEMS) & 1) ^ 1u, abort_flag, p.status, ST_WAIT_EMPTY)) return false;
+      const uint32_t ph = ((it / AX_ITEMS) & 1) ^ 1u;
+      if (!until([&] { return cl + AX_ITEMS > it && __all_sync(FULL_MASK, ax_test(&iempty[s], ph)); })) return false;
       if (lane == 0) {
         items[s] = x;
         mbar_arrive(&ifull[s]);
@@ -419,7 +487,8 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       return true;
     };
     if (u0 < u1) {
-      int head = static_cast<int>(u0 / C), b = *s_start, base = -32;
+      const long long before_me = cta > 0 ? bound(cta - 1) : 0;
+      int head = head0, b = *s_start, base = -32;
       long long off = *s_off, u = u0 - off;      // u: where the request's tiles begin
       int w_lo = 0, w_n = 0, w_sl = 0;           // a window of 32 requests, one per lane
       while (ok && u < u1) {
@@ -476,11 +545,11 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
               x.p0 = static_cast<int>(a - fp);
               x.p1 = static_cast<int>(z - fp);
               x.slot = x.p0 == 0 ? (x.p1 == pg ? -1 : 2 * cta + 1) : 2 * cta;
-              if (x.p0 > 0 && ((fp + 1) * n_eff - 1) / U == cta - 1) {   // the first cut of its tile: merged in this CTA's name
+              if (x.p0 > 0 && fp >= before_me) {     // the first cut of its tile: merged in this CTA's name
                 described = true;
                 if (lane == 0) {
                   int32_t* d = p.desc + cta * 8;
-                  d[0] = static_cast<int>((te * n_eff - 1) / U) - cta + 2;   // pieces
+                  d[0] = te <= u1 ? 2 : range_of(te - 1) - cta + 2;   // pieces
                   d[1] = x.tok0;
                   d[2] = nt;
                   d[3] = head;
@@ -498,8 +567,7 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     if (!described && lane == 0) p.desc[cta * 8] = 0;
     if (ok) {
       AxItem end{};
-      ok = push(end);
-      while (ok && cl < it - 1) ok = clear();
+      if (push(end)) until([&] { return cl == it; });
     }
   } else if (warp == 0) {
     // ---------------- K pages and Q tiles ----------------
@@ -576,7 +644,7 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     if (*abort_flag && lane == 0)   // a page on its tail barrier never counts as full now: its time runs out instead
       for (int i = max(0, issued - X::NV); i < issued; ++i) ax_drain(&vfull[i % X::NV], (i / X::NV) & 1);
   } else if (warp == 2) {
-    // ---------------- MMA issuer.  The score MMAs run two pages ahead of the P . V MMAs (also into the next item), so the
+    // ---------------- MMA issuer.  The score MMAs run NS pages ahead of the P . V MMAs (also into the next item), so the
     // tensor pipe has a product to do while the softmax warps work on a page.  P . V is issued per quarter of a page, as
     // its probabilities arrive ----------------
     const uint32_t q_lo = ax_desc_lo(smem_u32(smem)), k_lo = ax_desc_lo(smem_u32(smem + X::OFF_K)),
@@ -589,7 +657,7 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       n = __shfl_sync(FULL_MASK, items[it % AX_ITEMS].p1 - items[it % AX_ITEMS].p0, 0);
       return n > 0;
     };
-    int s_it = 0, s_i = 0, s_n = 0, ts = 0, k_st = 0, k_ph = 0;
+    int s_it = 0, s_i = 0, s_n = 0, s_b = 0, k_st = 0, k_ph = 0;
     bool s_more = true, ok = true;
     auto issue_s = [&]() {
       if (!s_more) return;
@@ -605,7 +673,7 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         }
         ++s_it;
       }
-      const uint32_t d = TM_S + (ts & 1) * 128;
+      const uint32_t d = TM_S + s_b * 128;
 #pragma unroll
       for (int u = 0; u < X::PU; ++u) {
         if (!ax_wait(&kfull[k_st], k_ph, abort_flag, p.status, ST_WAIT_FULL)) {
@@ -623,7 +691,7 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           }
           tc_commit(&kempty[k_st]);
           if (u == X::PU - 1) {
-            tc_commit(&sfull[ts & 1]);
+            tc_commit(&sfull[s_b]);
             if (s_i == s_n - 1) tc_commit(qempty);
           }
         }
@@ -633,15 +701,14 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           k_ph ^= 1;
         }
       }
-      ++ts;
+      s_b = s_b + 1 == X::NS ? 0 : s_b + 1;
       ++s_i;
     };
-    issue_s();
-    issue_s();
-    int it = 0, tp = 0, n = 0, v_st = 0, v_ph = 0;
+#pragma unroll 1
+    for (int i = 0; i < X::NS; ++i) issue_s();
+    int it = 0, n = 0, b = 0, b_ph = 0, v_st = 0, v_ph = 0;
     while (ok && get(it, n)) {
-      for (int i = 0; ok && i < n; ++i, ++tp) {
-        const int b = tp & 1;
+      for (int i = 0; ok && i < n; ++i) {
         const uint32_t pa = TM_S + b * 128;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {          // 32 keys each
@@ -649,7 +716,7 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             ok = ax_wait(&vfull[v_st], v_ph, abort_flag, p.status, ST_WAIT_FULL);
             if (!ok) break;
           }
-          ok = ax_wait(&pready[b * 4 + c], (tp >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
+          ok = ax_wait(&pready[b * 4 + c], b_ph, abort_flag, p.status, ST_WAIT_TMEM_FULL);
           if (ok && c == 0 && i == 0 && it > 0) ok = ax_wait(&ofree[(it - 1) % AX_ITEMS], ((it - 1) / AX_ITEMS) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY);
           if (!ok) break;
           tc_fence_after();
@@ -677,6 +744,10 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             v_ph ^= 1;
           }
         }
+        if (++b == X::NS) {
+          b = 0;
+          b_ph ^= 1;
+        }
         if (ok) issue_s();
       }
       ++it;
@@ -694,7 +765,6 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     const int q = warp & 3, e = (warp - AX_SOFT0) >> 2;
     const int row = q * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
-    const uint32_t sc = TM_S + e * 128 + lanes;
     const float sl2 = p.scale_log2;
     const int r_tok = row / p.grp, r_head = row - r_tok * p.grp;
     AxItem x;
@@ -707,13 +777,19 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       const bool active = q * 32 < x.ntok * p.grp;   // warps without a row only take part in the hand-overs
       const int lim = x.pos0 + r_tok;                // last key that this row sees
       const int32_t* tab = p.table + static_cast<size_t>(x.req) * p.pt_stride;
+      if (p.gate && x.slot < 0 && r_tok < x.ntok && x.tok0 + r_tok < p.T) {   // the epilogue's gate rows, on their way to L2
+        const bf16* g = p.gate + (x.tok0 + r_tok) * p.gate_stride + (x.head * p.grp + r_head) * D + e * (D / 2);
+#pragma unroll
+        for (int c = 0; c < D / 128; ++c) asm volatile("prefetch.global.L2 [%0];" ::"l"(g + c * 64));
+      }
       float m_own = -INFINITY, l = 0.f;              // the maximum that l is relative to
       uint32_t bad = 0;                              // missing pages among 32
       for (int i = (tp0 & 1) ^ e; ok && i < n; i += 2) {
-        const int tp = tp0 + i, pg = x.p0 + i;
+        const int tp = tp0 + i, pg = x.p0 + i, sb = tp % X::NS;
+        const uint32_t sc = TM_S + sb * 128 + lanes;
         if (!active) {
-          ok = ax_wait(&sfull[e], (tp >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
-          if (ok && lane < 4) mbar_arrive(&pready[e * 4 + lane]);
+          ok = ax_wait(&sfull[sb], (tp / X::NS) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
+          if (ok && lane < 4) mbar_arrive(&pready[sb * 4 + lane]);
           continue;
         }
         if ((i & 31) < 2) {
@@ -724,7 +800,7 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         const bool gone = (bad >> (i & 31)) & 1;
         const bool edge = gone || pg * AX_PAGE + AX_PAGE - 1 > x.pos0;   // not every row sees all of the page
         const int see = gone ? -1 : lim - pg * AX_PAGE;
-        ok = ax_wait(&sfull[e], (tp >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
+        ok = ax_wait(&sfull[sb], (tp / X::NS) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
         if (!ok) break;
         tc_fence_after();
         if (edge) {                                  // masked in place, so that the two passes below need not ask
@@ -773,9 +849,9 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           m_own = m_new;
           if (i > 0 && __any_sync(FULL_MASK, move)) {
             // P . V of the page before.  Its barrier's phase before is known to be over (the scores of page tp came after
-            // P . V of page tp - 2) and its next one cannot be (it needs this page), so the parity is not mistaken
+            // P . V of page tp - NS) and its next one cannot be (it needs this page), so the parity is not mistaken
             const float alpha = move ? ax_exp2((m - m_new) * sl2) : 1.f;
-            ok = ax_wait(&pvdone[e ^ 1], ((tp - 1) >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY);
+            ok = ax_wait(&pvdone[(tp - 1) % X::NS], ((tp - 1) / X::NS) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll 1
@@ -828,7 +904,7 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           ax_tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&pready[e * 4 + c]);
+          if (lane == 0) mbar_arrive(&pready[sb * 4 + c]);
         }
         l += (acc[0] + acc[1]) + (acc[2] + acc[3]);
       }
@@ -839,13 +915,8 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       const long long tok = x.tok0 + r_tok;
       const bool store = r_tok < x.ntok && tok < p.T;
       const int col0 = e * (D / 2);
-      uint4 gv[D / 16];
-      if (p.gate && store && x.slot < 0) {           // requested before the last P . V is waited for
-        const uint4* g = reinterpret_cast<const uint4*>(p.gate + tok * p.gate_stride + (x.head * p.grp + r_head) * D + col0);
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j) gv[j] = g[j];
-      }
-      if (mine) ok = ax_wait(&pvdone[e], (last >> 1) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
+      const uint32_t stored = __ballot_sync(FULL_MASK, store);
+      if (mine) ok = ax_wait(&pvdone[last % X::NS], (last / X::NS) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
       if (!ok) break;
       if (active) {
         pub += (n + ((tp0 & 1) ^ e)) >> 1;           // the other warp's pages: the larger half if it had the first
@@ -866,36 +937,70 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         tc_fence_after();
         const float total = l + s_l[(e ^ 1) * 128 + row];
         const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
-        bf16* o = p.out + (tok * p.hq + x.head * p.grp + r_head) * D + col0;
-        float* po = p.part + (static_cast<size_t>(max(x.slot, 0)) * p.rows + row) * D + col0;
+        if (x.slot >= 0) {                           // partial: [column / 4][row], a warp's rows side by side
+          float4* po = reinterpret_cast<float4*>(p.part) + (static_cast<size_t>(x.slot) * (D / 4) + col0 / 4) * p.rows + row;
+#pragma unroll 1
+          for (int c = 0; c < D / 64; ++c) {
+            uint32_t v[32];
+            tmem_ld32(TM_O + col0 + c * 32 + lanes, v);
+            tmem_ld_wait();
+            if (store) {
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          uint32_t v[32];
-          tmem_ld32(TM_O + col0 + c * 32 + lanes, v);
-          tmem_ld_wait();
-          if (store && x.slot >= 0) {
+              for (int j = 0; j < 8; ++j)
+                po[static_cast<size_t>(c * 8 + j) * p.rows] =
+                    make_float4(__uint_as_float(v[j * 4]), __uint_as_float(v[j * 4 + 1]), __uint_as_float(v[j * 4 + 2]),
+                                __uint_as_float(v[j * 4 + 3]));
+            }
+            __syncwarp();
+          }
+        } else {
+          // 64 columns at a time.  A lane owns a row, so its 16-byte pieces go through an 8 x 8 exchange among 8 lanes: then one
+          // access covers 4 rows of 128 bytes instead of 32 rows of 16 (the epilogue took 5 to 9 us with those)
+          const int sub = lane & 7;
+#pragma unroll 1
+          for (int c = 0; c < D / 128; ++c) {
+            uint4 g[8];
+            if (p.gate) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              reinterpret_cast<uint4*>(po + c * 32)[j] = make_uint4(v[j * 4], v[j * 4 + 1], v[j * 4 + 2], v[j * 4 + 3]);
-          } else if (store) {
+              for (int k = 0; k < 8; ++k) {
+                const int r = (lane & 24) + k;
+                const int rt = __shfl_sync(FULL_MASK, r_tok, r), rh = __shfl_sync(FULL_MASK, r_head, r);
+                if ((stored >> r) & 1)
+                  g[k] = *reinterpret_cast<const uint4*>(p.gate + (x.tok0 + rt) * p.gate_stride +
+                                                         (x.head * p.grp + rh) * D + col0 + c * 64 + sub * 8);
+              }
+              ax_exchange8(g, lane);
+            }
+            uint32_t v[64];
+            tmem_ld32(TM_O + col0 + c * 64 + lanes, *reinterpret_cast<uint32_t(*)[32]>(v));
+            tmem_ld32(TM_O + col0 + c * 64 + 32 + lanes, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
+            tmem_ld_wait();
+            uint4 o[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int k = 0; k < 8; ++k) {
               float f[8];
 #pragma unroll
-              for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(v[j * 8 + k]) * inv;
+              for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(v[k * 8 + j]) * inv;
               if (p.gate) {
-                const uint32_t gw[4] = {gv[c * 4 + j].x, gv[c * 4 + j].y, gv[c * 4 + j].z, gv[c * 4 + j].w};
+                const uint32_t gw[4] = {g[k].x, g[k].y, g[k].z, g[k].w};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  f[k * 2] = __fdividef(f[k * 2], 1.f + __expf(-bf_lo(gw[k])));
-                  f[k * 2 + 1] = __fdividef(f[k * 2 + 1], 1.f + __expf(-bf_hi(gw[k])));
+                for (int j = 0; j < 4; ++j) {
+                  f[j * 2] = __fdividef(f[j * 2], 1.f + __expf(-bf_lo(gw[j])));
+                  f[j * 2 + 1] = __fdividef(f[j * 2 + 1], 1.f + __expf(-bf_hi(gw[j])));
                 }
               }
-              reinterpret_cast<uint4*>(o + c * 32)[j] =
-                  make_uint4(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]), pack_bf2(f[4], f[5]), pack_bf2(f[6], f[7]));
+              o[k] = make_uint4(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]), pack_bf2(f[4], f[5]), pack_bf2(f[6], f[7]));
+            }
+            ax_exchange8(o, lane);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int r = (lane & 24) + k;
+              const int rt = __shfl_sync(FULL_MASK, r_tok, r), rh = __shfl_sync(FULL_MASK, r_head, r);
+              if ((stored >> r) & 1)
+                *reinterpret_cast<uint4*>(p.out + ((static_cast<long long>(x.tok0) + rt) * p.hq + x.head * p.grp + rh) * D + col0 +
+                                          c * 64 + sub * 8) = o[k];
             }
           }
-          __syncwarp();
         }
         if (x.slot >= 0 && store && e == 0) {
           float* ml = p.part + static_cast<size_t>(2 * grid) * p.rows * D + static_cast<size_t>(x.slot) * 2 * p.rows;
@@ -920,69 +1025,97 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   }
 }
 
-// Merge of the tiles whose pages were cut: the pieces are added in page order with weights 2^(m - M).  One CTA per (range
-// that a cut tile's second piece belongs to, 8 rows), one warp per row.
+// Merge of the tiles whose pages were cut: the pieces are added in page order with weights 2^(m - M), M the largest of their
+// maxima.  One CTA per (range that a cut tile's second piece belongs to, 32 rows); a lane owns a row, a warp an eighth of the
+// columns.  Where a tile has 8 or 16 rows (decode, where a long history is cut into many pieces) the lanes' groups share
+// the pieces between them and add up at the end, always in the same order.
+constexpr int AX_MAX_PIECES = 160;
 template <int D>
 __global__ void __launch_bounds__(256) attn_extend_merge_kernel(const AxArgs p, int grid) {
+  __shared__ float s_m[AX_MAX_PIECES][32], s_l[AX_MAX_PIECES][32];
   pdl_wait();
   pdl_launch();
   const int32_t* d = p.desc + blockIdx.x * 8;
-  const int pieces = d[0];
+  const int pieces = min(d[0], AX_MAX_PIECES);
   if (pieces <= 0) return;
   const int tok0 = d[1], ntok = d[2], head = d[3];
-  const int row = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int row0 = blockIdx.y * 32, left = ntok * p.grp - row0;        // rows of the tile from row0 on
+  if (left <= 0) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int span = left <= 8 ? 8 : left <= 16 ? 16 : 32;               // lanes per group
+  const int sub = lane / span, subs = 32 / span, r = lane % span, row = row0 + r;
   const int tok = tok0 + row / p.grp;
-  if (row >= ntok * p.grp || tok >= p.T) return;
-  const int first = 2 * (static_cast<int>(blockIdx.x) - 1) + 1;      // then 2 * blockIdx.x, 2 * (blockIdx.x + 1), ...
+  const bool live = r < left && tok < p.T;
+  const int first = 2 * (static_cast<int>(blockIdx.x) - 1) + 1;        // then 2 * blockIdx.x, 2 * (blockIdx.x + 1), ...
   auto slot = [&](int i) -> size_t { return i == 0 ? first : 2 * (blockIdx.x + i - 1); };
   const float* ml = p.part + static_cast<size_t>(2 * grid) * p.rows * D;
+  for (int i = warp * subs + sub; i < pieces; i += 8 * subs) {
+    s_m[i][r] = live ? ml[slot(i) * 2 * p.rows + row] : -INFINITY;
+    s_l[i][r] = live ? ml[slot(i) * 2 * p.rows + p.rows + row] : 0.f;
+  }
+  __syncthreads();
   float M = -INFINITY;
-  for (int i = lane; i < pieces; i += 32) M = fmaxf(M, ml[slot(i) * 2 * p.rows + row]);
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(FULL_MASK, M, o));
-  constexpr int V = D / 128;      // float4 per lane
+  for (int i = sub; i < pieces; i += subs) M = fmaxf(M, s_m[i][r]);
+  for (int o = span; o < 32; o <<= 1) M = fmaxf(M, __shfl_xor_sync(FULL_MASK, M, o));
+  constexpr int V = D / 32;      // float4s of a warp's columns
   float4 acc[V] = {};
   float L = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < pieces; ++i) {
-    const size_t s = slot(i);
-    const float m = ml[s * 2 * p.rows + row];
-    const float w = m == -INFINITY ? 0.f : ax_exp2(m - M);
-    L = fmaf(ml[s * 2 * p.rows + p.rows + row], w, L);
+  const float4* part = reinterpret_cast<const float4*>(p.part) + static_cast<size_t>(warp * V) * p.rows + row;
+#pragma unroll 2
+  for (int i = sub; i < pieces; i += subs) {
+    const float m = s_m[i][r], w = m == -INFINITY ? 0.f : ax_exp2(m - M);
+    L = fmaf(s_l[i][r], w, L);
+    const float4* x = part + slot(i) * (D / 4) * p.rows;
+    float4 v[V];
+#pragma unroll
+    for (int c = 0; c < V; ++c) v[c] = live ? x[static_cast<size_t>(c) * p.rows] : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int c = 0; c < V; ++c) {
-      const float4 v = reinterpret_cast<const float4*>(p.part + (s * p.rows + row) * D)[c * 32 + lane];
-      acc[c].x = fmaf(v.x, w, acc[c].x);
-      acc[c].y = fmaf(v.y, w, acc[c].y);
-      acc[c].z = fmaf(v.z, w, acc[c].z);
-      acc[c].w = fmaf(v.w, w, acc[c].w);
+      acc[c].x = fmaf(v[c].x, w, acc[c].x);
+      acc[c].y = fmaf(v[c].y, w, acc[c].y);
+      acc[c].z = fmaf(v[c].z, w, acc[c].z);
+      acc[c].w = fmaf(v[c].w, w, acc[c].w);
     }
   }
+  for (int o = span; o < 32; o <<= 1) {
+    L += __shfl_xor_sync(FULL_MASK, L, o);
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      acc[c].x += __shfl_xor_sync(FULL_MASK, acc[c].x, o);
+      acc[c].y += __shfl_xor_sync(FULL_MASK, acc[c].y, o);
+      acc[c].z += __shfl_xor_sync(FULL_MASK, acc[c].z, o);
+      acc[c].w += __shfl_xor_sync(FULL_MASK, acc[c].w, o);
+    }
+  }
+  if (!live || sub != 0) return;
   const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
-  const int hd = head * p.grp + row % p.grp;
+  const int hd = head * p.grp + row % p.grp, col = warp * V * 4;
+  const uint2* g = p.gate ? reinterpret_cast<const uint2*>(p.gate + tok * p.gate_stride + static_cast<long long>(hd) * D + col) : nullptr;
+  uint2* o = reinterpret_cast<uint2*>(p.out + (static_cast<long long>(tok) * p.hq + hd) * D + col);
 #pragma unroll
   for (int c = 0; c < V; ++c) {
-    const int col = (c * 32 + lane) * 4;
     float f[4] = {acc[c].x * inv, acc[c].y * inv, acc[c].z * inv, acc[c].w * inv};
-    if (p.gate) {
-      const uint2 g = *reinterpret_cast<const uint2*>(p.gate + tok * p.gate_stride + static_cast<long long>(hd) * D + col);
-      f[0] = __fdividef(f[0], 1.f + __expf(-bf_lo(g.x)));
-      f[1] = __fdividef(f[1], 1.f + __expf(-bf_hi(g.x)));
-      f[2] = __fdividef(f[2], 1.f + __expf(-bf_lo(g.y)));
-      f[3] = __fdividef(f[3], 1.f + __expf(-bf_hi(g.y)));
+    if (g) {
+      const uint2 gv = g[c];
+      f[0] = __fdividef(f[0], 1.f + __expf(-bf_lo(gv.x)));
+      f[1] = __fdividef(f[1], 1.f + __expf(-bf_hi(gv.x)));
+      f[2] = __fdividef(f[2], 1.f + __expf(-bf_lo(gv.y)));
+      f[3] = __fdividef(f[3], 1.f + __expf(-bf_hi(gv.y)));
     }
-    *reinterpret_cast<uint2*>(p.out + (static_cast<long long>(tok) * p.hq + hd) * D + col) =
-        make_uint2(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]));
+    o[c] = make_uint2(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]));
   }
 }
+
+static int ax_grid() { return sm_count() < AX_MAX_PIECES ? sm_count() : AX_MAX_PIECES; }
 
 template <bool F8, int D>
 static void ax_launch(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV, const AxArgs& a, cudaStream_t st) {
   using X = AxShape<F8, D>;
   static DeviceOnce once;
   once.run([] { cudaFuncSetAttribute(attn_extend_kernel<F8, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, X::SMEM); });
-  const int grid = sm_count();
+  const int grid = ax_grid();
   launch_k(attn_extend_kernel<F8, D>, dim3(grid), dim3(AX_THREADS), X::SMEM, st, tmQ, tmK, tmV, a);
-  launch_k(attn_extend_merge_kernel<D>, dim3(grid, (a.rows + 7) / 8), dim3(256), 0, st, a, grid);
+  launch_k(attn_extend_merge_kernel<D>, dim3(grid, (a.rows + 31) / 32), dim3(256), 0, st, a, grid);
 }
 
 // rows of a tile: the group's heads of as many tokens as fit 128 rows, or of all T
@@ -997,7 +1130,7 @@ using namespace b200;
 
 extern "C" size_t b200_attn_extend_workspace_bytes(int T, int Hq, int Hkv, int D) {
   if (T <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || Hq % Hkv || Hq / Hkv > 128) return 0;
-  const size_t rows = static_cast<size_t>(ax_tokens_per_tile(T, Hq / Hkv)) * (Hq / Hkv), grid = sm_count();
+  const size_t rows = static_cast<size_t>(ax_tokens_per_tile(T, Hq / Hkv)) * (Hq / Hkv), grid = ax_grid();
   return grid * 32 + 2 * grid * rows * (static_cast<size_t>(D) + 2) * 4;
 }
 
@@ -1056,7 +1189,7 @@ extern "C" int b200_attn_extend(const void* q, long long q_stride, const void* g
   a.scale_log2 = scale * 1.4426950408889634f;
   a.out = static_cast<bf16*>(out);
   a.desc = static_cast<int32_t*>(ws);
-  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + static_cast<size_t>(sm_count()) * 32);
+  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + static_cast<size_t>(ax_grid()) * 32);
   a.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (cache_bf16)
