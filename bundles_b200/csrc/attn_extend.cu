@@ -29,8 +29,8 @@ namespace b200 {
 B200_DEFINE_WAIT_BUDGET_SETTER(set_wait_budget_attn_extend)
 
 constexpr int AX_PAGE = 128;
-constexpr int AX_OVH = 2;              // cost of a tile beside its pages, in pages
-constexpr int AX_MIN_UNITS = 4;        // smallest range worth a CTA of its own
+constexpr int AX_OVH = 4;              // cost of a tile beside its pages, in pages
+constexpr int AX_MIN_UNITS = 2;        // smallest range worth a CTA of its own
 constexpr float AX_BIAS = 8.f;         // log2 scale of the 8-bit probabilities
 constexpr float AX_TAU = 4.f;          // log2 distance that moves the running maximum: 2^(8 + 4) fits both formats
 constexpr int AX_ITEMS = 4;            // ring of work items
@@ -178,27 +178,6 @@ __device__ __forceinline__ void ax_add2(float& a, float& b, float c, float d) {
   asm("{\n.reg .b64 x, y;\nmov.b64 x, {%0, %1};\nmov.b64 y, {%2, %3};\nadd.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}\n"
       : "+f"(a), "+f"(b)
       : "f"(c), "f"(d));
-}
-// 8 x 8 transposition of 16-byte pieces among 8 neighbouring lanes: piece k of lane b becomes piece b of lane k
-__device__ __forceinline__ void ax_exchange8(uint4 (&x)[8], int lane) {
-#pragma unroll
-  for (int o = 4; o > 0; o >>= 1) {
-    const bool up = (lane & o) != 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if ((k & o) == 0) {
-        const uint4 send = up ? x[k] : x[k | o];
-        uint4 got;
-        got.x = __shfl_xor_sync(FULL_MASK, send.x, o);
-        got.y = __shfl_xor_sync(FULL_MASK, send.y, o);
-        got.z = __shfl_xor_sync(FULL_MASK, send.z, o);
-        got.w = __shfl_xor_sync(FULL_MASK, send.w, o);
-        if (up)
-          x[k] = got;
-        else
-          x[k | o] = got;
-      }
-  }
 }
 __device__ __forceinline__ void ax_tma_load_3d(void* smem_dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
@@ -915,7 +894,12 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       const long long tok = x.tok0 + r_tok;
       const bool store = r_tok < x.ntok && tok < p.T;
       const int col0 = e * (D / 2);
-      const uint32_t stored = __ballot_sync(FULL_MASK, store);
+      uint4 gv[D / 16];
+      if (p.gate && store && x.slot < 0) {           // requested before the last P . V is waited for
+        const uint4* g = reinterpret_cast<const uint4*>(p.gate + tok * p.gate_stride + (x.head * p.grp + r_head) * D + col0);
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) gv[j] = g[j];
+      }
       if (mine) ok = ax_wait(&pvdone[last % X::NS], (last / X::NS) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
       if (!ok) break;
       if (active) {
@@ -954,52 +938,31 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             __syncwarp();
           }
         } else {
-          // 64 columns at a time.  A lane owns a row, so its 16-byte pieces go through an 8 x 8 exchange among 8 lanes: then one
-          // access covers 4 rows of 128 bytes instead of 32 rows of 16 (the epilogue took 5 to 9 us with those)
-          const int sub = lane & 7;
-#pragma unroll 1
-          for (int c = 0; c < D / 128; ++c) {
-            uint4 g[8];
-            if (p.gate) {
+          bf16* o = p.out + (tok * p.hq + x.head * p.grp + r_head) * D + col0;
 #pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                const int r = (lane & 24) + k;
-                const int rt = __shfl_sync(FULL_MASK, r_tok, r), rh = __shfl_sync(FULL_MASK, r_head, r);
-                if ((stored >> r) & 1)
-                  g[k] = *reinterpret_cast<const uint4*>(p.gate + (x.tok0 + rt) * p.gate_stride +
-                                                         (x.head * p.grp + rh) * D + col0 + c * 64 + sub * 8);
-              }
-              ax_exchange8(g, lane);
-            }
-            uint32_t v[64];
-            tmem_ld32(TM_O + col0 + c * 64 + lanes, *reinterpret_cast<uint32_t(*)[32]>(v));
-            tmem_ld32(TM_O + col0 + c * 64 + 32 + lanes, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
+          for (int c = 0; c < D / 64; ++c) {
+            uint32_t v[32];
+            tmem_ld32(TM_O + col0 + c * 32 + lanes, v);
             tmem_ld_wait();
-            uint4 o[8];
+            if (store) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              float f[8];
+              for (int j = 0; j < 4; ++j) {
+                float f[8];
 #pragma unroll
-              for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(v[k * 8 + j]) * inv;
-              if (p.gate) {
-                const uint32_t gw[4] = {g[k].x, g[k].y, g[k].z, g[k].w};
+                for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(v[j * 8 + k]) * inv;
+                if (p.gate) {
+                  const uint32_t gw[4] = {gv[c * 4 + j].x, gv[c * 4 + j].y, gv[c * 4 + j].z, gv[c * 4 + j].w};
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  f[j * 2] = __fdividef(f[j * 2], 1.f + __expf(-bf_lo(gw[j])));
-                  f[j * 2 + 1] = __fdividef(f[j * 2 + 1], 1.f + __expf(-bf_hi(gw[j])));
+                  for (int k = 0; k < 4; ++k) {
+                    f[k * 2] = __fdividef(f[k * 2], 1.f + __expf(-bf_lo(gw[k])));
+                    f[k * 2 + 1] = __fdividef(f[k * 2 + 1], 1.f + __expf(-bf_hi(gw[k])));
+                  }
                 }
+                reinterpret_cast<uint4*>(o + c * 32)[j] =
+                    make_uint4(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]), pack_bf2(f[4], f[5]), pack_bf2(f[6], f[7]));
               }
-              o[k] = make_uint4(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]), pack_bf2(f[4], f[5]), pack_bf2(f[6], f[7]));
             }
-            ax_exchange8(o, lane);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const int r = (lane & 24) + k;
-              const int rt = __shfl_sync(FULL_MASK, r_tok, r), rh = __shfl_sync(FULL_MASK, r_head, r);
-              if ((stored >> r) & 1)
-                *reinterpret_cast<uint4*>(p.out + ((static_cast<long long>(x.tok0) + rt) * p.hq + x.head * p.grp + rh) * D + col0 +
-                                          c * 64 + sub * 8) = o[k];
-            }
+            __syncwarp();
           }
         }
         if (x.slot >= 0 && store && e == 0) {
