@@ -204,15 +204,16 @@ __device__ __forceinline__ long long ax_floor_sum(uint32_t m, uint32_t d, uint32
   }
   return r;
 }
-// x / y, in 32 bits where both fit
-__device__ __forceinline__ long long ax_div(long long x, long long y) {
+// x / y, in 32 bits where both fit.  This and the costs below stay out of line: a CTA runs them a few times at its start, when
+// every instruction line is a miss
+__device__ __noinline__ long long ax_div(long long x, long long y) {
   if (((x | y) >> 32) == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(y);
   return x / y;
 }
 // pages that a tile reads whose last token sees keys 0 .. end - 1
 __device__ __forceinline__ int ax_pages(int end) { return end <= 0 ? 0 : (end + AX_PAGE - 1) / AX_PAGE; }
 // cost of a request's first k tiles, all of tpt tokens; ctx: keys before its first new token (negative: missing)
-__device__ __forceinline__ long long ax_cost(int k, int ctx, int tpt) {
+__device__ __noinline__ long long ax_cost(int k, int ctx, int tpt) {
   const int skip = ctx < 0 ? min(k, -ctx / tpt) : 0;   // tiles whose last token sees nothing
   return static_cast<long long>(k) * AX_OVH +
          ax_floor_sum(k - skip, AX_PAGE, tpt, static_cast<uint32_t>(ctx + (skip + 1) * tpt + AX_PAGE - 1));
@@ -322,6 +323,7 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   const int cta = blockIdx.x, grid = gridDim.x;
   const int per = (p.B + AX_THREADS - 1) / AX_THREADS, b0 = min(p.B, static_cast<int>(threadIdx.x) * per), b1 = min(p.B, b0 + per);
   long long mine = 0;
+#pragma unroll 1
   for (int b = b0; b < b1; ++b) {
     const int n = p.cu[b + 1] - p.cu[b];
     mine += ax_cost_all(n, p.seqlens[b] - n, p.tpt);
@@ -357,16 +359,16 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     const long long v0 = u0 - head0 * C;
     if (v0 >= before && v0 < before + mine) {
       long long at = before;
-      for (int b = b0; b < b1; ++b) {
+      int b = b0;
+#pragma unroll 1
+      for (; b < b1 - 1; ++b) {      // the last one needs no look
         const int n = p.cu[b + 1] - p.cu[b];
         const long long c = ax_cost_all(n, p.seqlens[b] - n, p.tpt);
-        if (v0 < at + c) {
-          *s_start = b;
-          *s_off = v0 - at;
-          break;
-        }
+        if (v0 < at + c) break;
         at += c;
       }
+      *s_start = b;
+      *s_off = v0 - at;
     }
   }
   fence_proxy_async();
@@ -782,34 +784,28 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         ok = ax_wait(&sfull[sb], (tp / X::NS) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
         if (!ok) break;
         tc_fence_after();
-        if (edge) {                                  // masked in place, so that the two passes below need not ask
-#pragma unroll 1
-          for (int c = 0; c < 8; ++c) {
-            uint32_t v[16];
-            tmem_ld16(sc + c * 16, v);
-            tmem_ld_wait();
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (c * 16 + j > see) v[j] = 0xff800000u;
-            ax_tmem_st16(sc + c * 16, v);
-          }
-          ax_tmem_st_wait();
-        }
         // the loops over a row's scores stay rolled: unrolled, a page's code overran the instruction cache, and the warps
         // waited for instructions a quarter of the time
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
-        for (int g = 0; g < 2; ++g) {
-          uint32_t s[64];
-          tmem_ld32(sc + g * 64, *reinterpret_cast<uint32_t(*)[32]>(s));
-          tmem_ld32(sc + g * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
+        for (int c = 0; c < 128; c += 32) {
+          uint32_t v[32];
+          tmem_ld32(sc + c, v);
           tmem_ld_wait();
+          if (edge) {                                // masked in place, so that the second pass need not ask
 #pragma unroll
-          for (int j = 0; j < 64; j += 8) {
+            for (int j = 0; j < 32; ++j)
+              if (c + j > see) v[j] = 0xff800000u;
+            ax_tmem_st16(sc + c, v);
+            ax_tmem_st16(sc + c + 16, v + 16);
+          }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) mx[k] = ax_max3(mx[k], __uint_as_float(s[j + k]), __uint_as_float(s[j + 4 + k]));
+          for (int j = 0; j < 32; j += 8) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mx[k] = ax_max3(mx[k], __uint_as_float(v[j + k]), __uint_as_float(v[j + 4 + k]));
           }
         }
+        if (edge) ax_tmem_st_wait();
         const float tm = fmaxf(ax_max3(mx[0], mx[1], mx[2]), mx[3]);
         // the maximum so far, of the page before
         float m = -INFINITY;
@@ -894,11 +890,12 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       const long long tok = x.tok0 + r_tok;
       const bool store = r_tok < x.ntok && tok < p.T;
       const int col0 = e * (D / 2);
-      uint4 gv[D / 16];
-      if (p.gate && store && x.slot < 0) {           // requested before the last P . V is waited for
-        const uint4* g = reinterpret_cast<const uint4*>(p.gate + tok * p.gate_stride + (x.head * p.grp + r_head) * D + col0);
+      uint4 gv[4];
+      const bool gated = p.gate && store && x.slot < 0;
+      const uint4* g = reinterpret_cast<const uint4*>(p.gate + (gated ? tok * p.gate_stride + (x.head * p.grp + r_head) * D + col0 : 0));
+      if (gated) {                                   // the first columns' gate, requested before the last P . V is waited for
 #pragma unroll
-        for (int j = 0; j < D / 16; ++j) gv[j] = g[j];
+        for (int j = 0; j < 4; ++j) gv[j] = g[j];
       }
       if (mine) ok = ax_wait(&pvdone[last % X::NS], (last / X::NS) & 1, abort_flag, p.status, ST_WAIT_TMEM_FULL);
       if (!ok) break;
@@ -939,10 +936,17 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           }
         } else {
           bf16* o = p.out + (tok * p.hq + x.head * p.grp + r_head) * D + col0;
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < D / 64; ++c) {
             uint32_t v[32];
             tmem_ld32(TM_O + col0 + c * 32 + lanes, v);
+            uint4 gc[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) gc[j] = gv[j];
+            if (gated && c + 1 < D / 64) {           // the next columns' gate
+#pragma unroll
+              for (int j = 0; j < 4; ++j) gv[j] = g[(c + 1) * 4 + j];
+            }
             tmem_ld_wait();
             if (store) {
 #pragma unroll
@@ -951,7 +955,7 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 #pragma unroll
                 for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(v[j * 8 + k]) * inv;
                 if (p.gate) {
-                  const uint32_t gw[4] = {gv[c * 4 + j].x, gv[c * 4 + j].y, gv[c * 4 + j].z, gv[c * 4 + j].w};
+                  const uint32_t gw[4] = {gc[j].x, gc[j].y, gc[j].z, gc[j].w};
 #pragma unroll
                   for (int k = 0; k < 4; ++k) {
                     f[k * 2] = __fdividef(f[k * 2], 1.f + __expf(-bf_lo(gw[k])));

@@ -167,8 +167,9 @@ __global__ void __launch_bounds__(PP_THREADS) page_plan_kernel(const PlanArgs p)
   }
 }
 
-// The append copies K rows as they are and turns V rows into columns of the dim-major pages.  A CTA takes the tokens that fill
-// 128 bytes of a page's V row (KA_TOK) and 64 dims of one kv head.  The tokens are cut into pieces that share one aligned
+// The append copies K rows as they are and turns V rows into columns of the dim-major pages.  A CTA takes KA_TOK tokens and 64 dims of
+// one kv head: the tokens that fill 128 bytes of a page's V row, or 16 where that would leave most of the GPU idle (64
+// decoded tokens: 8 CTAs, 7.6 us; 32 CTAs, 3.0 us).  The tokens are cut into pieces that share one aligned
 // 16-byte chunk of a page (a new piece starts where the slots do not follow on, and at every chunk); eight neighbouring
 // lanes take neighbouring pieces of the same dims, so whole pages are written in full 128-byte lines.  A piece that is not
 // a whole chunk (a lone decoded token) is written element by element.  V passes through shared memory in 4-byte words
@@ -176,12 +177,12 @@ __global__ void __launch_bounds__(PP_THREADS) page_plan_kernel(const PlanArgs p)
 // Bound: HBM for prompts; the two dependent loads (slot, row) and the launch for a decode step.
 constexpr int KA_DIMS = 64, KA_THREADS = 128;
 
-template <typename E>
+template <typename E, int KA_TOK>
 __global__ void __launch_bounds__(KA_THREADS) kv_append_kernel(const E* __restrict__ k, const E* __restrict__ v,
                                                                long long k_stride, long long v_stride, int T, int hkv, int dim,
                                                                E* __restrict__ kc, E* __restrict__ vc, int num_pages,
                                                                const int64_t* __restrict__ slots, int32_t* status) {
-  constexpr int ES = sizeof(E), KA_TOK = 128 / ES, G = 16 / ES;   // tokens of the tile, of a chunk
+  constexpr int ES = sizeof(E), G = 16 / ES;                       // tokens of a chunk
   constexpr int ROW_W = KA_DIMS * ES / 4, ROW_Q = KA_DIMS * ES / 16;   // words and 16-byte quarters of a token's slice
   constexpr int PER_W = 4 / ES;                                    // dims of a word
   __shared__ long long s_slot[KA_TOK];
@@ -206,7 +207,7 @@ __global__ void __launch_bounds__(KA_THREADS) kv_append_kernel(const E* __restri
   }
   if (tid < KA_TOK) s_slot[tid] = slot;
   // both tiles are requested before the slots are looked at
-  constexpr int LD = KA_TOK * ROW_Q / KA_THREADS;
+  constexpr int LD = (KA_TOK * ROW_Q + KA_THREADS - 1) / KA_THREADS;
   uint4 kr[LD], vr[LD];
 #pragma unroll
   for (int i = 0; i < LD; ++i) {
@@ -281,6 +282,14 @@ __global__ void __launch_bounds__(KA_THREADS) kv_append_kernel(const E* __restri
   }
 }
 
+template <typename E, int WIDE>
+static void ka_launch(bool narrow, unsigned grid, const void* k, const void* v, long long ks, long long vs, int T, int hkv, int dim,
+                      void* kc, void* vc, int pages, const int64_t* slots, int32_t* status, cudaStream_t st) {
+  launch_k(narrow ? kv_append_kernel<E, 16> : kv_append_kernel<E, WIDE>, dim3(grid), dim3(KA_THREADS), 0, st,
+           static_cast<const E*>(k), static_cast<const E*>(v), ks, vs, T, hkv, dim, static_cast<E*>(kc), static_cast<E*>(vc), pages,
+           slots, status);
+}
+
 }  // namespace b200
 
 using namespace b200;
@@ -324,15 +333,15 @@ extern "C" int b200_kv_append(const void* k, const void* v, long long k_stride, 
     return fail(B200_E_ALIGN, "b200_kv_append: tensors and token strides must be 16-byte aligned");
   if (T == 0) return 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const long long tok = cache_bf16 ? 64 : 128, grid = (T + tok - 1) / tok * Hkv * (D / KA_DIMS);
+  const long long wide = cache_bf16 ? 64 : 128, cols = static_cast<long long>(Hkv) * (D / KA_DIMS);
+  const bool narrow = (T + wide - 1) / wide * cols < sm_count() / 2;
+  const long long grid = (narrow ? (T + 15) / 16 : (T + wide - 1) / wide) * cols;
   if (grid > 0x7fffffffll) return fail(B200_E_ARG, "b200_kv_append: too many tokens (T=%d)", T);
   if (cache_bf16)
-    launch_k(kv_append_kernel<uint16_t>, dim3(static_cast<unsigned>(grid)), dim3(KA_THREADS), 0, st,
-             static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), k_stride, v_stride, T, Hkv, D,
-             static_cast<uint16_t*>(kcache), static_cast<uint16_t*>(vcache), num_pages, slots, status);
+    ka_launch<uint16_t, 64>(narrow, static_cast<unsigned>(grid), k, v, k_stride, v_stride, T, Hkv, D, kcache, vcache, num_pages,
+                            slots, status, st);
   else
-    launch_k(kv_append_kernel<uint8_t>, dim3(static_cast<unsigned>(grid)), dim3(KA_THREADS), 0, st,
-             static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v), k_stride, v_stride, T, Hkv, D,
-             static_cast<uint8_t*>(kcache), static_cast<uint8_t*>(vcache), num_pages, slots, status);
+    ka_launch<uint8_t, 128>(narrow, static_cast<unsigned>(grid), k, v, k_stride, v_stride, T, Hkv, D, kcache, vcache, num_pages,
+                            slots, status, st);
   return launch_status("b200_kv_append");
 }
