@@ -223,6 +223,14 @@ __device__ __forceinline__ long long ax_cost_all(int n, int ctx, int tpt) {
   return ax_cost((n - 1) / tpt, ctx, tpt) + AX_OVH + ax_pages(ctx + n);
 }
 
+// Request b: its rows lo .. lo + n - 1 and the keys before its first new token, from lengths that may be anything: rows are kept
+// inside [0, T), keys behind the block table are missing anyway and do not count
+__device__ __forceinline__ void ax_request(const AxArgs& p, int b, int& lo, int& n, int& ctx) {
+  lo = min(max(p.cu[b], 0), p.T);
+  n = min(max(p.cu[b + 1], 0), p.T) - lo;
+  ctx = min(max(p.seqlens[b], 0) - n, p.pt_stride * AX_PAGE);
+}
+
 // Waits of a whole warp: every lane polls, and all give up together.  The wait proper stays out of line: most barriers are
 // complete when they are asked for, and the MMA issuer's own instructions have to fit between its MMAs.
 __device__ __noinline__ bool ax_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
@@ -255,7 +263,11 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   using X = AxShape<F8, D>;
   extern __shared__ __align__(1024) uint8_t smem[];   // the swizzled tiles start on 1024 bytes; there is no room for slack
   if (smem_u32(smem) & 1023u) {
-    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, ST_WAIT_STATE);
+    pdl_wait();
+    if (threadIdx.x == 0) {
+      p.desc[blockIdx.x * 8] = 0;
+      if (p.status) atomicCAS(p.status, 0, ST_WAIT_STATE);
+    }
     return;
   }
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + X::OFF_BAR);
@@ -325,8 +337,9 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   long long mine = 0;
 #pragma unroll 1
   for (int b = b0; b < b1; ++b) {
-    const int n = p.cu[b + 1] - p.cu[b];
-    mine += ax_cost_all(n, p.seqlens[b] - n, p.tpt);
+    int lo, n, ctx;
+    ax_request(p, b, lo, n, ctx);
+    mine += ax_cost_all(n, ctx, p.tpt);
   }
   long long inc = mine;
 #pragma unroll
@@ -362,8 +375,9 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       int b = b0;
 #pragma unroll 1
       for (; b < b1 - 1; ++b) {      // the last one needs no look
-        const int n = p.cu[b + 1] - p.cu[b];
-        const long long c = ax_cost_all(n, p.seqlens[b] - n, p.tpt);
+        int lo, n, ctx;
+        ax_request(p, b, lo, n, ctx);
+        const long long c = ax_cost_all(n, ctx, p.tpt);
         if (v0 < at + c) break;
         at += c;
       }
@@ -471,7 +485,7 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       const long long before_me = cta > 0 ? bound(cta - 1) : 0;
       int head = head0, b = *s_start, base = -32;
       long long off = *s_off, u = u0 - off;      // u: where the request's tiles begin
-      int w_lo = 0, w_n = 0, w_sl = 0;           // a window of 32 requests, one per lane
+      int w_lo = 0, w_n = 0, w_ctx = 0;          // a window of 32 requests, one per lane
       while (ok && u < u1) {
         if (b >= p.B) {
           b = 0;
@@ -479,13 +493,11 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         }
         if (b < base || b >= base + 32 || base < 0) {
           base = b;
-          const int r = min(b + lane, p.B - 1);
-          w_lo = p.cu[r];
-          w_n = b + lane < p.B ? p.cu[r + 1] - w_lo : 0;
-          w_sl = p.seqlens[r];
+          ax_request(p, min(b + lane, p.B - 1), w_lo, w_n, w_ctx);
+          if (b + lane >= p.B) w_n = 0;
         }
         const int lo = __shfl_sync(FULL_MASK, w_lo, b - base), n = __shfl_sync(FULL_MASK, w_n, b - base);
-        const int ctx = __shfl_sync(FULL_MASK, w_sl, b - base) - n;
+        const int ctx = __shfl_sync(FULL_MASK, w_ctx, b - base);
         if (n <= 0) {
           ++b;
           continue;
@@ -1108,9 +1120,9 @@ extern "C" int b200_attn_extend(const void* q, long long q_stride, const void* g
                                 int32_t* status, void* stream) {
   if (!q || !kcache || !vcache || !page_table || !cu_seqlens || !seqlens || !out || !ws)
     return fail(B200_E_ARG, "b200_attn_extend: null pointer");
-  if (B <= 0 || B > 8192 || T <= 0 || T > (1 << 24) || num_pages <= 0 || pt_stride <= 0)
-    return fail(B200_E_ARG, "b200_attn_extend: need 1 <= B <= 8192, 1 <= T <= 2^24, num_pages and pt_stride >= 1 (B=%d T=%d)",
-                B, T);
+  if (B <= 0 || B > 8192 || T <= 0 || T > (1 << 24) || num_pages <= 0 || pt_stride <= 0 || pt_stride > (1 << 23))
+    return fail(B200_E_ARG, "b200_attn_extend: need 1 <= B <= 8192, 1 <= T <= 2^24, num_pages >= 1 and 1 <= pt_stride <= 2^23 "
+                "(B=%d T=%d)", B, T);
   if (Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq / Hkv > 128 || Hkv > 128 || (D != 128 && D != 256))
     return fail(B200_E_ARG, "b200_attn_extend: need Hq a multiple of Hkv, at most 128 heads per group, D 128 or 256 "
                 "(Hq=%d Hkv=%d D=%d)", Hq, Hkv, D);

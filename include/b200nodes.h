@@ -379,7 +379,9 @@ int b200_attn_verify(const void* q, const void* gate, const void* k_new, const v
  *   q e4m3 or bf16 as the cache, [T, Hq, D] with a token stride in elements; out bf16 [T, Hq * D].
  *   A row that sees no key is written as zeros; rows behind cu_seqlens[B] are left as they are; keys on missing pages
  *   are masked (B200_ST_BAD_PAGE).  Keys behind a request's last token may hold anything, NaN included.
- *   cu_seqlens[0] = 0 and ascending, seqlens >= 0.  scale > 0.
+ *   cu_seqlens ascends from 0 (values outside [0, T] are clamped; a request that would run backwards has no rows, and no two
+ *   requests may share one); seqlens below 0 count as 0.  scale > 0 and finite.  B <= 8192, T <= 2^24, pt_stride <= 2^23,
+ *   at most 128 query heads per kv head.
  *   ws: b200_attn_extend_workspace_bytes(T, Hq, Hkv, D) bytes, 16-byte aligned, one per call in flight.
  */
 int b200_page_plan(const int32_t* ctx_lens, const int32_t* new_lens, int B, int32_t* page_table, int pt_stride,

@@ -224,3 +224,91 @@ def test_pool_past_four_gigabytes():
     out = ops.attn_extend(**c, scale=scale)
     torch.cuda.synchronize()
     pu.check(out, d, scale)
+
+
+def test_lengths_that_are_nonsense_stay_in_bounds():
+    """Row bounds outside [0, T), a request that runs backwards, lengths below zero and far beyond the table: the sound rows are
+    right, the clamped ones are written inside the output, nothing else is."""
+    from bundles_b200 import ops
+    d, scale = pu.make([(6, 200), (4, 30), (10, 90)], seed=23)
+    c = pu.on(d, DEV)
+    whole = ops.attn_extend(**c, scale=scale)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    out = torch.full_like(whole, 7.0)
+    c["cu_seqlens"] = torch.tensor([-50, 6, 3, 20], **i32)         # rows 0..5, none, 3..19: the last two requests lie
+    c["seqlens"] = torch.tensor([206, -2147483648, 100], **i32)
+    c["cu_seqlens"][3] = 3                                          # ... the last has none either
+    ops.attn_extend(**c, scale=scale, out=out)
+    torch.cuda.synchronize()
+    assert torch.equal(out[:6], whole[:6]) and (out[6:] == 7.0).all()
+    c["cu_seqlens"] = torch.tensor([0, 6, 10, 2147483647], **i32)   # the last request's rows end with the buffer
+    c["seqlens"] = torch.tensor([206, 34, 100], **i32)
+    ops.attn_extend(**c, scale=scale, out=out)
+    torch.cuda.synchronize()
+    assert torch.equal(out, whole)
+    c["seqlens"] = torch.tensor([2147483647, -5, 2147483647], **i32)  # everything in the table is seen; nothing is
+    ops.attn_extend(**c, scale=scale, out=out)
+    torch.cuda.synchronize()
+    assert torch.isnan(out[:6]).all() and (out[6:10] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["e4m3", "bf16"])
+@pytest.mark.parametrize("heads", [(16, 2, 256), (12, 4, 128)])
+def test_back_to_back_calls_of_changing_shape(dtype, heads):
+    """Calls of many shapes in a row on one stream, every output as from a call alone: items of one page between long ones,
+    warps without rows, cut and whole tiles."""
+    from bundles_b200 import ops
+    sets = []
+    for k, b in enumerate(([(1, 60)] * 40, [(1, 5000)], [(300, 10)], [(1, 0), (90, 1000), (1, 127)], [(2, 64)] * 7)):
+        d, scale = pu.make(b, dtype, heads, seed=60 + k)
+        sets.append(pu.on(d, DEV))
+    status = ops.new_status(DEV)
+    alone = []
+    for c in sets:
+        alone.append(ops.attn_extend(**c, scale=scale))
+        torch.cuda.synchronize()
+    for _ in range(20):
+        outs = [ops.attn_extend(**c, scale=scale, status=status) for c in sets]
+    torch.cuda.synchronize()
+    assert ops.read_status(status) == 0
+    assert all(torch.equal(a, b) for a, b in zip(outs, alone))
+
+
+def test_two_streams_at_once():
+    from bundles_b200 import ops
+    cases = [pu.make([(1, 3000), (70, 200)], seed=70 + k)[0] for k in range(2)]
+    dev = [pu.on(d, DEV) for d in cases]
+    want = [ops.attn_extend(**c) for c in dev]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(ops.attn_extend(**dev[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(o, want[k]) for o in got[k])
+
+
+def test_refusals_of_tensors_that_do_not_fit():
+    from bundles_b200 import ops
+    d, _ = pu.make([(3, 140)], seed=80)
+    c = pu.on(d, DEV)
+
+    def bad(match, **kw):
+        with pytest.raises(ops.B200Error, match=match):
+            ops.attn_extend(**{**c, **kw})
+    bad("must be", q=c["q"].to(torch.bfloat16))
+    bad("must be", q=c["q"][:, :, :128].contiguous())
+    bad("contiguous", q=c["q"].transpose(0, 1).contiguous().transpose(0, 1))
+    bad("row per token", gate=c["gate"][:2])
+    bad("fit together", cu_seqlens=c["cu_seqlens"][:1].contiguous())
+    bad("CUDA", seqlens=c["seqlens"].cpu())
+    bad("CUDA", page_table=c["page_table"].cpu())
+    bad("K \\[pages", vcache=c["vcache"].transpose(2, 3).contiguous())
+    bad("out must be", out=torch.empty(3, 4000, dtype=torch.bfloat16, device=DEV))
+    bad("code -1", scale=0.0)
+    bad("code -3", ws=torch.empty(64, dtype=torch.uint8, device=DEV))
+    bad("code -2", q=torch.zeros(3 * 4096 + 1, dtype=torch.uint8, device=DEV)[1:].view(3, 16, 256))
+    assert ops.attn_extend(c["q"][:0], c["gate"][:0], *[c[n] for n in ("kcache", "vcache", "page_table", "cu_seqlens", "seqlens")]).shape == (0, 4096)

@@ -45,7 +45,7 @@ def test_attn_extend_refusals(lib):
         return lib.b200_attn_extend(q, qs, gate, gs, kc, one, P, one, W, one, one, B, T, hq, hkv, D, bf16, scale, out, ws, n, None,
                                     None)
     for bad in (dict(q=None), dict(kc=None), dict(out=None), dict(ws=None), dict(B=0), dict(B=8193), dict(T=0), dict(T=(1 << 24) + 1),
-                dict(P=0), dict(W=0), dict(hq=15), dict(hq=0), dict(hkv=0), dict(hq=258, hkv=2, qs=1 << 17, gs=1 << 17),
+                dict(P=0), dict(W=0), dict(W=(1 << 23) + 1), dict(hq=15), dict(hq=0), dict(hkv=0), dict(hq=258, hkv=2, qs=1 << 17, gs=1 << 17),
                 dict(D=64), dict(P=1 << 23), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")),
                 dict(qs=4095), dict(gs=4000)):
         assert call(**bad) == -1, bad
