@@ -54,6 +54,7 @@ struct AxArgs {
   int32_t* desc;                 // [grid][8]: tiles to merge
   float* part;                   // [2 * grid][D / 4][rows][4] unnormalised, then [2 * grid][2][rows]: maximum, row sum
   int rows;                      // tpt * grp
+  int sub;                       // tokens of a small Q box: their rows fill whole groups of 8
   int32_t* status;
 };
 
@@ -258,8 +259,8 @@ __device__ __forceinline__ void ax_drain(uint64_t* bar, uint32_t parity) {
 
 template <bool F8, int D>
 __global__ void __launch_bounds__(AX_THREADS, 1)
-attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                   const __grid_constant__ CUtensorMap tmV, const AxArgs p) {
+attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmQs,
+                   const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const AxArgs p) {
   using X = AxShape<F8, D>;
   extern __shared__ __align__(1024) uint8_t smem[];   // the swizzled tiles start on 1024 bytes; there is no room for slack
   if (smem_u32(smem) & 1023u) {
@@ -328,6 +329,7 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     tma_prefetch_desc(&tmV);
   }
   if (warp == 2) tmem_alloc(tmem_slot, 512);
+  for (int i = threadIdx.x; i < X::QB / 16; i += AX_THREADS) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
   pdl_wait();
   pdl_launch();
 
@@ -572,8 +574,18 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       if (it > 0) ok = ax_wait(qempty, (it - 1) & 1, abort_flag, p.status, ST_WAIT_EMPTY);
       if (!ok) break;
       if (lane == 0) {
-        mbar_expect_tx(qfull, X::NB * p.rows * 128);
-        for (int c = 0; c < X::NB; ++c) ax_tma_load_3d(smem + c * 16384, &tmQ, c * 128, x.head * p.grp, x.tok0, qfull);
+        // A tile of few tokens gets only their rows: the others stay zero (or an earlier item's), and products of zeros take less
+        // power, which is what limits the clock here (64 x 8192 tokens of decode, sustained: 117 us with full boxes, 114 so)
+        const int boxes = (x.ntok + p.sub - 1) / p.sub;
+        if (boxes * p.sub * 2 <= p.tpt) {
+          mbar_expect_tx(qfull, X::NB * boxes * p.sub * p.grp * 128);
+          for (int t = 0; t < boxes; ++t)
+            for (int c = 0; c < X::NB; ++c)
+              ax_tma_load_3d(smem + c * 16384 + t * p.sub * p.grp * 128, &tmQs, c * 128, x.head * p.grp, x.tok0 + t * p.sub, qfull);
+        } else {
+          mbar_expect_tx(qfull, X::NB * p.rows * 128);
+          for (int c = 0; c < X::NB; ++c) ax_tma_load_3d(smem + c * 16384, &tmQ, c * 128, x.head * p.grp, x.tok0, qfull);
+        }
       }
       int ids = 0;
       for (int j = x.p0; ok && j < x.p1; ++j) {
@@ -853,7 +865,8 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             }
           }
         }
-        const float shift = (F8 ? AX_BIAS : 0.f) - (m_new == -INFINITY ? 0.f : m_new * sl2);
+        // rows of no token get zero probabilities (see the Q boxes)
+        const float shift = r_tok < x.ntok ? (F8 ? AX_BIAS : 0.f) - (m_new == -INFINITY ? 0.f : m_new * sl2) : -INFINITY;
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
@@ -1088,12 +1101,12 @@ __global__ void __launch_bounds__(256) attn_extend_merge_kernel(const AxArgs p, 
 static int ax_grid() { return sm_count() < AX_MAX_PIECES ? sm_count() : AX_MAX_PIECES; }
 
 template <bool F8, int D>
-static void ax_launch(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV, const AxArgs& a, cudaStream_t st) {
+static void ax_launch(const CUtensorMap& tmQ, const CUtensorMap& tmQs, const CUtensorMap& tmK, const CUtensorMap& tmV, const AxArgs& a, cudaStream_t st) {
   using X = AxShape<F8, D>;
   static DeviceOnce once;
   once.run([] { cudaFuncSetAttribute(attn_extend_kernel<F8, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, X::SMEM); });
   const int grid = ax_grid();
-  launch_k(attn_extend_kernel<F8, D>, dim3(grid), dim3(AX_THREADS), X::SMEM, st, tmQ, tmK, tmV, a);
+  launch_k(attn_extend_kernel<F8, D>, dim3(grid), dim3(AX_THREADS), X::SMEM, st, tmQ, tmQs, tmK, tmV, a);
   launch_k(attn_extend_merge_kernel<D>, dim3(grid, (a.rows + 31) / 32), dim3(256), 0, st, a, grid);
 }
 
@@ -1139,7 +1152,7 @@ extern "C" int b200_attn_extend(const void* q, long long q_stride, const void* g
   if (ws_bytes < b200_attn_extend_workspace_bytes(T, Hq, Hkv, D))
     return fail(B200_E_WS, "b200_attn_extend: workspace %zu < %zu bytes", ws_bytes,
                 b200_attn_extend_workspace_bytes(T, Hq, Hkv, D));
-  CUtensorMap tmQ, tmK, tmV;
+  CUtensorMap tmQ, tmQs, tmK, tmV;
   int rc;
   AxArgs a{};
   a.grp = Hq / Hkv;
@@ -1147,6 +1160,11 @@ extern "C" int b200_attn_extend(const void* q, long long q_stride, const void* g
   a.rows = a.tpt * a.grp;
   if ((rc = make_tmap_bytes_3d(&tmQ, q, static_cast<uint64_t>(D) * es, Hq, T, static_cast<uint64_t>(D) * es,
                                static_cast<uint64_t>(q_stride) * es, a.grp, a.tpt, "q")))
+    return rc;
+  a.sub = a.grp % 8 == 0 ? 1 : a.grp % 4 == 0 ? 2 : a.grp % 2 == 0 ? 4 : 8;
+  if (a.sub > a.tpt) a.sub = a.tpt;   // never used then: two such boxes do not fit the tile
+  if ((rc = make_tmap_bytes_3d(&tmQs, q, static_cast<uint64_t>(D) * es, Hq, T, static_cast<uint64_t>(D) * es,
+                               static_cast<uint64_t>(q_stride) * es, a.grp, a.sub, "q")))
     return rc;
   if ((rc = make_tmap_bytes_2d(&tmK, kcache, static_cast<uint64_t>(num_pages) * Hkv * AX_PAGE, static_cast<uint64_t>(D) * es,
                                AX_PAGE, "k cache")))
@@ -1172,8 +1190,8 @@ extern "C" int b200_attn_extend(const void* q, long long q_stride, const void* g
   a.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (cache_bf16)
-    D == 256 ? ax_launch<false, 256>(tmQ, tmK, tmV, a, st) : ax_launch<false, 128>(tmQ, tmK, tmV, a, st);
+    D == 256 ? ax_launch<false, 256>(tmQ, tmQs, tmK, tmV, a, st) : ax_launch<false, 128>(tmQ, tmQs, tmK, tmV, a, st);
   else
-    D == 256 ? ax_launch<true, 256>(tmQ, tmK, tmV, a, st) : ax_launch<true, 128>(tmQ, tmK, tmV, a, st);
+    D == 256 ? ax_launch<true, 256>(tmQ, tmQs, tmK, tmV, a, st) : ax_launch<true, 128>(tmQ, tmQs, tmK, tmV, a, st);
   return launch_status("b200_attn_extend");
 }
