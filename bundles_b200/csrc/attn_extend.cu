@@ -8,19 +8,35 @@
 //
 // Rows.  The query heads of one kv head share its keys, so a tile's 128 rows are (token, head of the group) pairs of one
 // request: 128 / group tokens at a time.  Q . K^T and P . V run on tcgen05 with the rows on the M side; a softmax thread
-// owns one row and half of the page's 128 keys, so a row's maximum and sum need one exchange between two warps.
+// owns a whole row of a page's scores, so its maximum and sum need no exchange, and the running maximum passes from the
+// warp of one page to the warp of the next.
 //
 // P in 8 bits.  With e4m3 pages V is the B operand of an 8-bit MMA as it lies in the page, which saves the conversion
-// of V to f16 (64 KB of shared memory and three passes over it per page) and half of the tensor time of a 16-bit product
-// for each of the two terms that P is given in: an e5m2 value h of P 2^AX_BIAS and the e4m3 value of the remainder
-// P 2^AX_BIAS - h.  h is within 2^(e-3) of a probability in [2^e, 2^(e+1)) and the remainder's own rounding within
-// 2^(e-8): half a step of 2^-8, what bf16 has.  The range: the remainder is a normal number for probabilities down to
-// 2^-11 of the maximum, h alone down to 2^-22 and, as a subnormal, 2^-25.  With bf16 pages P is bf16.
+// of V to f16 (64 KB of shared memory and three passes over it per page) at the tensor time of one 16-bit product: P is
+// given in two terms, an e5m2 value h of P 2^AX_BIAS and the e4m3 value of the remainder P 2^AX_BIAS - h.  h is within
+// 2^(e-3) of a probability in [2^e, 2^(e+1)) and the remainder's own rounding within 2^(e-8): half a step of 2^-8, what
+// bf16 has.  The range: the remainder is a normal number for probabilities down to 2^-11 of the maximum, h alone down to
+// 2^-22 and, as a subnormal, 2^-25.  With bf16 pages P is bf16.  Error against 64 bits, 2-norm: 2.1e-3 (e4m3) and 2.3e-3
+// (bf16), of which the output's own rounding to bf16 is 1.7e-3.
 //
 // Work.  Every (kv head, request, tile) costs its pages plus AX_OVH; the sequence of all of them is cut into equal
 // ranges, one per CTA, so that a batch of any shape fills the GPU.  Every CTA finds its range from the lengths by itself
 // (a closed form for the pages of a request's first k tiles), so nothing is planned on the host and a captured graph may
 // be replayed with other lengths.
+//
+// What bounds it.  Prompts: a page costs the tensor pipe 1536 cycles (D = 256, e4m3: 512 for the scores, 1024 for the two
+// terms of P . V) and takes about 2150.  The score buffers are the link: they and the accumulator fill the 512 columns of
+// TMEM, so the scores of page t + NS wait for P . V of page t, and half of (softmax of a page, about 2600 cycles, + P . V,
+// scores and hand-overs, about 1700) is what a page takes with two buffers.  The exponential unit is busy 1024 of those.
+// Four 2048-token chunks behind 6144 tokens: 0.60 ms at first and 0.70 ms sustained (1545 MHz under the power limit),
+// 1.4 PFLOP/s.  Decode: 64 requests x 8192 tokens, 0.54 GB of e4m3 pages: 100 us, 114 us sustained (1440 MHz) = 4.7 TB/s.
+// Tried and dropped: four softmax warps per scheduler, each with half of a page (607 -> 650 us: more instructions, no
+// shorter chain); a quarter of the exponentials as a cubic on the FMA pipe (605 -> 610 us); polling instead of suspended
+// waits (650 -> 687 us: the pollers take the issue slots); 8 x 8 exchanges between lanes for an epilogue that writes whole
+// lines (mixed step 106 -> 119 us).
+//
+// A NaN or an infinity in V reaches every row of a tile that holds a row which sees it (a zero probability times it is NaN);
+// what no row of the tile sees is cleared or never loaded.
 #include "common.cuh"
 #include "host.h"
 
@@ -29,8 +45,10 @@ namespace b200 {
 B200_DEFINE_WAIT_BUDGET_SETTER(set_wait_budget_attn_extend)
 
 constexpr int AX_PAGE = 128;
-constexpr int AX_OVH = 4;              // cost of a tile beside its pages, in pages
-constexpr int AX_MIN_UNITS = 2;        // smallest range worth a CTA of its own
+constexpr int AX_OVH = 4;              // cost of a tile beside its pages, in pages (a mixed step with 2 / 4 / 6 / 8: 118 / 96 /
+                                       // 94 / 100 us; chunks of 1000 to 1500 bf16 tokens: 104 / 106 / 108 / 128 us)
+constexpr int AX_MIN_UNITS = 2;        // smallest range worth a CTA of its own (one token, 8192 keys, with 1 / 2 / 4: 25.8 / 19.7 /
+                                       // 20.3 us: more pieces cost the merge more than they save)
 constexpr float AX_BIAS = 8.f;         // log2 scale of the 8-bit probabilities
 constexpr float AX_TAU = 4.f;          // log2 distance that moves the running maximum: 2^(8 + 4) fits both formats
 constexpr int AX_ITEMS = 4;            // ring of work items
@@ -83,7 +101,6 @@ struct AxShape {
   static constexpr int SMEM = OFF_RED + 2 * 2 * 128 * 4;
   static_assert(SMEM <= 232448, "shared memory of a CTA");
   static constexpr int VBOX = D * 128;                 // one V box: D rows of 128 bytes
-  static constexpr int NVB = ES;                       // boxes per V page
   static constexpr int NS = D == 128 ? 3 : 2;          // score buffers: what the accumulator leaves of 512 columns
   static_assert((2 * NK + 3 * NV + 3 * AX_ITEMS + 6 * NS + 14) * 8 + 24 <= 640, "room for the barriers");
 };
@@ -280,14 +297,14 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   uint64_t* iempty = ifull + AX_ITEMS;    // [AX_ITEMS] all roles are done with it
   uint64_t* sfull = iempty + AX_ITEMS;    // [NS] scores complete in TMEM
   uint64_t* pready = sfull + X::NS;       // [NS][4 quarters] probabilities written (and O rescaled if needed)
-  uint64_t* mpub = pready + 4 * X::NS;            // [2 page parities][4 quadrants] running maximum published
+  uint64_t* mpub = pready + 4 * X::NS;    // [2 page parities][4 quadrants] running maximum published
   uint64_t* lpub = mpub + 8;              // [4] both warps' row sums published, the last P . V done
   uint64_t* qfull = lpub + 4;             // Q tile landed
   uint64_t* qempty = qfull + 1;           // the item's last score MMA is done
   uint64_t* pvdone = qempty + 1;          // [NS] P . V of a page done
-  uint64_t* ofree = pvdone + X::NS;           // [AX_ITEMS] the item's accumulator has been read (by ring place: a warp without rows
+  uint64_t* ofree = pvdone + X::NS;       // [AX_ITEMS] the item's accumulator has been read (by ring place: a warp without rows
                                           // may be some items ahead, and must not arrive twice in one phase)
-  uint64_t* vtail = ofree + AX_ITEMS;            // [NV] V page with places behind the last key landed
+  uint64_t* vtail = ofree + AX_ITEMS;     // [NV] V page with places behind the last key landed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(vtail + X::NV);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_start = reinterpret_cast<int*>(tmem_slot + 2);   // request
@@ -722,7 +739,8 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             if (!ok) break;
           }
           ok = ax_wait(&pready[b * 4 + c], b_ph, abort_flag, p.status, ST_WAIT_TMEM_FULL);
-          if (ok && c == 0 && i == 0 && it > 0) ok = ax_wait(&ofree[(it - 1) % AX_ITEMS], ((it - 1) / AX_ITEMS) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY);
+          if (ok && c == 0 && i == 0 && it > 0)
+            ok = ax_wait(&ofree[(it - 1) % AX_ITEMS], ((it - 1) / AX_ITEMS) & 1, abort_flag, p.status, ST_WAIT_TMEM_EMPTY);
           if (!ok) break;
           tc_fence_after();
           const uint32_t vb = v_lo + v_st * (X::UNIT >> 4);
