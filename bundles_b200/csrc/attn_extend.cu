@@ -34,9 +34,6 @@
 // shorter chain); a quarter of the exponentials as a cubic on the FMA pipe (605 -> 610 us); polling instead of suspended
 // waits (650 -> 687 us: the pollers take the issue slots); 8 x 8 exchanges between lanes for an epilogue that writes whole
 // lines (mixed step 106 -> 119 us).
-//
-// A NaN or an infinity in V reaches every row of a tile that holds a row which sees it (a zero probability times it is NaN);
-// what no row of the tile sees is cleared or never loaded.
 #include "common.cuh"
 #include "host.h"
 
@@ -61,6 +58,7 @@ struct AxArgs {
   long long q_stride;
   const bf16* gate;
   long long gate_stride;
+  const void* vc;
   int num_pages;
   const int32_t* table;
   int pt_stride;
@@ -82,6 +80,9 @@ struct AxItem {
   int pos0, p0, p1, slot;        // pos0: its place in the request; slot: partial slot or -1
 };
 
+// the first of an item's pages that not every row of its tile sees to the end
+__device__ __forceinline__ int ax_first_edge(const AxItem& x) { return max(x.p0, (max(x.pos0, -1) + 1) / AX_PAGE); }
+
 template <bool F8, int D>
 struct AxShape {
   static constexpr int ES = F8 ? 1 : 2;
@@ -96,13 +97,13 @@ struct AxShape {
   static constexpr int OFF_K = QB;
   static constexpr int OFF_V = OFF_K + NK * UNIT;
   static constexpr int OFF_BAR = OFF_V + NV * UNIT;
-  static constexpr int OFF_ITEM = OFF_BAR + 640;   // barriers and 24 bytes
+  static constexpr int OFF_ITEM = OFF_BAR + 640;       // barriers and 40 bytes
   static constexpr int OFF_RED = OFF_ITEM + AX_ITEMS * 32;
   static constexpr int SMEM = OFF_RED + 2 * 2 * 128 * 4;
   static_assert(SMEM <= 232448, "shared memory of a CTA");
   static constexpr int VBOX = D * 128;                 // one V box: D rows of 128 bytes
   static constexpr int NS = D == 128 ? 3 : 2;          // score buffers: what the accumulator leaves of 512 columns
-  static_assert((2 * NK + 3 * NV + 3 * AX_ITEMS + 6 * NS + 14) * 8 + 24 <= 640, "room for the barriers");
+  static_assert((2 * NK + 3 * NV + 3 * AX_ITEMS + 6 * NS + 14) * 8 + 40 <= 640, "room for the barriers");
 };
 
 __device__ __forceinline__ uint32_t ax_sw128(int row, int chunk) {
@@ -241,12 +242,54 @@ __device__ __forceinline__ long long ax_cost_all(int n, int ctx, int tpt) {
   return ax_cost((n - 1) / tpt, ctx, tpt) + AX_OVH + ax_pages(ctx + n);
 }
 
+// mask of the first n bytes of a word
+__device__ __forceinline__ uint32_t ax_below(int n) { return n >= 4 ? ~0u : n <= 0 ? 0u : ~0u >> (32 - n * 8); }
+// mask of the e4m3 or bf16 elements of a word that are NaN or infinite
+template <bool F8>
+__device__ __forceinline__ uint32_t ax_not_finite(uint32_t w) {
+  return F8 ? ((((w & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u) * 0xffu
+            : ((((w & 0x7f807f80u) + 0x00800080u) >> 15) & 0x00010001u) * 0xffffu;
+}
+
 // Request b: its rows lo .. lo + n - 1 and the keys before its first new token, from lengths that may be anything: rows are kept
 // inside [0, T), keys behind the block table are missing anyway and do not count
 __device__ __forceinline__ void ax_request(const AxArgs& p, int b, int& lo, int& n, int& ctx) {
   lo = min(max(p.cu[b], 0), p.T);
   n = min(max(p.cu[b + 1], 0), p.T) - lo;
   ctx = min(max(p.seqlens[b], 0) - n, p.pt_stride * AX_PAGE);
+}
+
+// What is not finite in the V of the keys that were cleared for a tile goes back to a row that sees them: NaN, or an infinity
+// of either sign, in the columns where it stood.  Runs for the tiles that hold such a value only.
+template <bool F8, int D>
+__device__ __forceinline__ void ax_give_back(const AxArgs& p, const AxItem& x, int row, int lim, long long tok, int hd, int col0) {
+  asm volatile("" ::: "memory");
+#pragma unroll 1
+  for (int d = col0; d < col0 + D / 2; ++d) {
+    float odd = 0.f;
+#pragma unroll 1
+    for (int j = max(x.pos0 + 1, x.p0 * AX_PAGE); j <= min(lim, x.p1 * AX_PAGE - 1); ++j) {
+      const int id = j / AX_PAGE < p.pt_stride ? p.table[static_cast<size_t>(x.req) * p.pt_stride + j / AX_PAGE] : -1;
+      if (id < 0 || id >= p.num_pages) continue;
+      const size_t at = ((static_cast<size_t>(id) * p.hkv + x.head) * D + d) * AX_PAGE + j % AX_PAGE;
+      if (F8) {
+        if ((static_cast<const uint8_t*>(p.vc)[at] & 0x7f) == 0x7f) odd = __int_as_float(0x7fffffff);
+      } else {
+        const float v = bf2f(static_cast<const bf16*>(p.vc)[at]);
+        if (!isfinite(v)) odd += v;
+      }
+    }
+    if (odd == 0.f) continue;
+    // added to what this thread has just stored there, which may be infinite already
+    if (x.slot >= 0) {
+      float* o = p.part + ((static_cast<size_t>(x.slot) * (D / 4) + d / 4) * p.rows + row) * 4 + d % 4;
+      *o = __ldcg(o) + odd;
+    } else {
+      if (p.gate) odd = odd / (1.f + __expf(-bf2f(p.gate[tok * p.gate_stride + static_cast<long long>(hd) * D + d])));
+      unsigned short* o = reinterpret_cast<unsigned short*>(p.out + (tok * p.hq + hd) * D + d);
+      *o = __bfloat16_as_ushort(f2bf(bf2f(__ushort_as_bfloat16(__ldcg(o))) + odd));
+    }
+  }
 }
 
 // Waits of a whole warp: every lane polls, and all give up together.  The wait proper stays out of line: most barriers are
@@ -304,11 +347,12 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   uint64_t* pvdone = qempty + 1;          // [NS] P . V of a page done
   uint64_t* ofree = pvdone + X::NS;       // [AX_ITEMS] the item's accumulator has been read (by ring place: a warp without rows
                                           // may be some items ahead, and must not arrive twice in one phase)
-  uint64_t* vtail = ofree + AX_ITEMS;     // [NV] V page with places behind the last key landed
+  uint64_t* vtail = ofree + AX_ITEMS;     // [NV] V page that has to be tended landed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(vtail + X::NV);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_start = reinterpret_cast<int*>(tmem_slot + 2);   // request
   long long* s_off = reinterpret_cast<long long*>(tmem_slot + 4);
+  volatile int* s_odd = reinterpret_cast<volatile int*>(tmem_slot + 6);   // [AX_ITEMS] values that are not finite were cleared
   AxItem* items = reinterpret_cast<AxItem*>(smem + X::OFF_ITEM);
   float* s_m = reinterpret_cast<float*>(smem + X::OFF_RED);   // [2 page parities][128 rows] running maximum
   float* s_l = s_m + 256;                                     // [2 page parities][128 rows] row sum
@@ -423,50 +467,68 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   };
 
   if (warp == 3) {
-    // ---------------- scheduler: walks the tiles of this CTA's range.  The same warp clears, in the copy of the last V page
-    // of an item, the places behind the last key that its tile sees: they may hold anything, and a zero probability
-    // times a NaN would spoil the row.  Such a page lands on a barrier of its own and counts as full once it is cleared; it is
-    // tended whenever it lands, also while a place in the item ring is waited for ----------------
-    int it = 0, cl = 0, cu = 0, pages = 0;   // items written; items cleared, units of the next one; pages of the cleared ones
+    // ---------------- scheduler: walks the tiles of this CTA's range.  The same warp tends the copies of the V pages that not
+    // every row of their tile sees to the end.  A zero probability times a NaN or an infinity would spoil a row, so the places
+    // behind the last key are cleared (they may hold anything), and so is what is not finite in the keys that some rows see
+    // and others do not; the epilogue then gives it back to the rows that see it.  Such a page lands on a barrier of its own
+    // and counts as full once it is tended; it is tended whenever it lands, also while a place in the item ring is waited for
+    int it = 0, cl = 0, ce = 0, cu = 0, pages = 0;   // items written; items tended, pages and units of the next; their pages
     uint32_t tails = 0;                      // per stage: phase of its tail barrier
     bool ok = true, described = false;
-    auto tend = [&]() -> bool {              // clears the next such unit if it has landed
+    auto tend = [&]() -> bool {              // the next such unit, if it has landed
       if (cl == it) return false;
       const AxItem x = items[cl % AX_ITEMS];
-      const int last = x.pos0 + x.ntok - (x.p1 - 1) * AX_PAGE;
-      if (last < AX_PAGE) {
-        const int st = ((pages + x.p1 - x.p0 - 1) * X::PU + cu) % X::NV;
+      const int j = ax_first_edge(x) + ce;
+      if (j < x.p1) {
+        const int st = ((pages + j - x.p0) * X::PU + cu) % X::NV;
         if (!__all_sync(FULL_MASK, ax_test(&vtail[st], (tails >> st) & 1))) return false;
         tails ^= 1u << st;
+        uint32_t found = 0;
 #pragma unroll 1
         for (int c = 0; c < X::UNIT / X::VBOX; ++c) {
-          const int vb = min(128, max(0, last * X::ES - (cu * (X::UNIT / X::VBOX) + c) * 128));   // valid bytes of a row of the box
+          // bytes of a row of the box: from `lo` on not every row of the tile sees them, from `hi` on none does
+          const int at = j * AX_PAGE * X::ES + (cu * (X::UNIT / X::VBOX) + c) * 128;
+          const int lo = min(128, max(0, (x.pos0 + 1) * X::ES - at)), hi = min(128, max(0, (x.pos0 + x.ntok) * X::ES - at));
           uint8_t* box = smem + X::OFF_V + st * X::UNIT + c * X::VBOX;
 #pragma unroll 1
-          for (int ch = vb >> 4; ch < 8; ++ch) {
-            uint4 keep;                      // bytes of the chunk that are valid
-            keep.x = vb - ch * 16 >= 4 ? ~0u : vb - ch * 16 <= 0 ? 0u : 0xffffffffu >> (32 - (vb - ch * 16) * 8);
-            keep.y = vb - ch * 16 >= 8 ? ~0u : vb - ch * 16 <= 4 ? 0u : 0xffffffffu >> (32 - (vb - ch * 16 - 4) * 8);
-            keep.z = vb - ch * 16 >= 12 ? ~0u : vb - ch * 16 <= 8 ? 0u : 0xffffffffu >> (32 - (vb - ch * 16 - 8) * 8);
-            keep.w = vb - ch * 16 >= 16 ? ~0u : vb - ch * 16 <= 12 ? 0u : 0xffffffffu >> (32 - (vb - ch * 16 - 12) * 8);
-#pragma unroll 4
+          for (int ch = lo >> 4; ch < 8; ++ch) {
+            if (ch * 16 >= hi) {
+#pragma unroll
+              for (int d = 0; d < D; d += 32) *reinterpret_cast<uint4*>(box + ax_sw128(d + lane, ch)) = make_uint4(0, 0, 0, 0);
+              continue;
+            }
+            uint32_t keep[4], look[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              keep[k] = ax_below(hi - ch * 16 - k * 4);
+              look[k] = keep[k] & ~ax_below(lo - ch * 16 - k * 4);
+            }
+#pragma unroll 2
             for (int d = lane; d < D; d += 32) {
               uint4* w = reinterpret_cast<uint4*>(box + ax_sw128(d, ch));
               uint4 v = *w;
-              v.x &= keep.x;
-              v.y &= keep.y;
-              v.z &= keep.z;
-              v.w &= keep.w;
-              *w = v;
+              uint32_t e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t odd = ax_not_finite<F8>(e[k]) & look[k];
+                found |= odd;
+                e[k] &= keep[k] & ~odd;
+              }
+              *w = make_uint4(e[0], e[1], e[2], e[3]);
             }
           }
         }
+        if (__any_sync(FULL_MASK, found != 0) && lane == 0) s_odd[cl % AX_ITEMS] = 1;
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(&vfull[st]);
-        if (++cu < X::PU) return true;
+        if (++cu == X::PU) {
+          cu = 0;
+          ++ce;
+        }
+        return true;
       }
-      cu = 0;
+      ce = 0;
       pages += x.p1 - x.p0;
       ++cl;
       return true;
@@ -494,6 +556,7 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       if (!until([&] { return cl + AX_ITEMS > it && __all_sync(FULL_MASK, ax_test(&iempty[s], ph)); })) return false;
       if (lane == 0) {
         items[s] = x;
+        s_odd[s] = 0;
         mbar_arrive(&ifull[s]);
       }
       __syncwarp();
@@ -648,7 +711,7 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         }
         const int id = __shfl_sync(FULL_MASK, ids, (j - x.p0) & 31);
         const int y = id < 0 || id >= p.num_pages ? p.num_pages * p.hkv * D : (id * p.hkv + x.head) * D;
-        uint64_t* full = x.pos0 + x.ntok < (j + 1) * AX_PAGE ? vtail : vfull;   // keys of the page end before it does
+        uint64_t* full = j >= ax_first_edge(x) ? vtail : vfull;
         for (int u = 0; u < X::PU; ++u, ++un) {
           const int st = un % X::NV;
           ok = ax_wait(&vempty[st], ((un / X::NV) & 1) ^ 1u, abort_flag, p.status, ST_WAIT_EMPTY);
@@ -1012,6 +1075,7 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             __syncwarp();
           }
         }
+        if (s_odd[it % AX_ITEMS] && store) ax_give_back<F8, D>(p, x, row, lim, tok, x.head * p.grp + r_head, col0);
         if (x.slot >= 0 && store && e == 0) {
           float* ml = p.part + static_cast<size_t>(2 * grid) * p.rows * D + static_cast<size_t>(x.slot) * 2 * p.rows;
           ml[row] = m * sl2;
@@ -1192,6 +1256,7 @@ extern "C" int b200_attn_extend(const void* q, long long q_stride, const void* g
   a.q_stride = q_stride;
   a.gate = static_cast<const bf16*>(gate);
   a.gate_stride = gate_stride;
+  a.vc = vcache;
   a.num_pages = num_pages;
   a.table = page_table;
   a.pt_stride = pt_stride;

@@ -378,8 +378,7 @@ int b200_attn_verify(const void* q, const void* gate, const void* k_new, const v
  *   out[t, h] = sigmoid(gate[t, h]) * softmax(scale * q . K) V in bf16, rounded once; gate bf16 or NULL (no gate).
  *   q e4m3 or bf16 as the cache, [T, Hq, D] with a token stride in elements; out bf16 [T, Hq * D].
  *   A row that sees no key is written as zeros; rows behind cu_seqlens[B] are left as they are; keys on missing pages
- *   are masked (B200_ST_BAD_PAGE).  Keys behind a request's last token may hold anything, NaN included; a NaN or
- *   infinity in V of a token in the batch reaches the rows of the same request within 128 / (Hq / Hkv) tokens before it.
+ *   are masked (B200_ST_BAD_PAGE).  Keys that a row does not see may hold anything, NaN included.
  *   cu_seqlens ascends from 0 (values outside [0, T] are clamped; a request that would run backwards has no rows, and no two
  *   requests may share one); seqlens below 0 count as 0.  scale > 0 and finite.  B <= 8192, T <= 2^24, pt_stride <= 2^23,
  *   at most 128 query heads per kv head.

@@ -312,3 +312,29 @@ def test_refusals_of_tensors_that_do_not_fit():
     bad("code -3", ws=torch.empty(64, dtype=torch.uint8, device=DEV))
     bad("code -2", q=torch.zeros(3 * 4096 + 1, dtype=torch.uint8, device=DEV)[1:].view(3, 16, 256))
     assert ops.attn_extend(c["q"][:0], c["gate"][:0], *[c[n] for n in ("kcache", "vcache", "page_table", "cu_seqlens", "seqlens")]).shape == (0, 4096)
+
+
+@pytest.mark.parametrize("gate", [True, False])
+@pytest.mark.parametrize("heads,dtype", [((16, 2, 256), "e4m3"), ((16, 2, 256), "bf16"), ((12, 4, 128), "e4m3"), ((4, 4, 128), "bf16")])
+def test_values_that_are_not_finite_reach_the_rows_that_see_them_only(heads, dtype, gate):
+    """NaN and infinities in K and V of new tokens in the middle of a chunk: the rows before them are as the formula says, those
+    from them on are not finite where the formula says so.  Whole tiles and cut ones, keys on two pages."""
+    d, scale = pu.make([(40, 100), (150, 1900), (3, 126)], dtype, heads, gate=gate, seed=90)
+    one = (lambda v: 0x7f) if dtype == "e4m3" else (lambda v: v)      # e4m3 has NaN only
+    inf, nan = float("inf"), float("nan")
+    for b, pos, dim, v in ((0, 127, 5, nan), (0, 128, 17, inf), (0, 135, 17, -inf), (1, 1910, 100, inf), (1, 1919, 3, nan),
+                           (1, 2049, 64, -inf), (2, 128, 127, nan)):
+        page = int(d["page_table"][b, pos // 128])
+        d["vcache"][page, :, dim, pos % 128] = one(v)
+    d["kcache"][int(d["page_table"][1, 2040 // 128]), :, 2040 % 128, 9] = one(nan)
+    out, st = _run(d, scale)
+    assert st == 0
+    with np.errstate(all="ignore"):
+        ref, spread = pu.want(d, scale)
+    got = out.float().cpu().numpy().astype(np.float64).reshape(ref.shape)
+    assert np.array_equal(np.isnan(got), np.isnan(ref)) and np.array_equal(np.isinf(got), np.isinf(ref))
+    assert np.array_equal(np.sign(got[np.isinf(got)]), np.sign(ref[np.isinf(ref)]))
+    fine = np.isfinite(ref)
+    assert fine.mean() > 0.5 and not fine.all()
+    err = np.abs(got[fine] - ref[fine])
+    assert (err <= 2.0 ** -8 * np.abs(ref[fine]) + 2.125 * 2.0 ** -8 * spread[fine]).all()
