@@ -1100,13 +1100,13 @@ attn_extend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 }
 
 // Merge of the tiles whose pages were cut: the pieces are added in page order with weights 2^(m - M), M the largest of their
-// maxima.  One CTA per (range that a cut tile's second piece belongs to, 32 rows); a lane owns a row, a warp an eighth of the
-// columns.  Where a tile has 8 or 16 rows (decode, where a long history is cut into many pieces) the lanes' groups share
+// maxima.  One CTA per (range that a cut tile's second piece belongs to, 32 rows, 128 columns); a lane owns a row, a warp 16 of
+// the columns.  Where a tile has 8 or 16 rows (decode, where a long history is cut into many pieces) the lanes' groups share
 // the pieces between them and add up at the end, always in the same order.
 constexpr int AX_MAX_PIECES = 160;
 template <int D>
-__global__ void __launch_bounds__(256) attn_extend_merge_kernel(const AxArgs p, int grid) {
-  __shared__ float s_m[AX_MAX_PIECES][32], s_l[AX_MAX_PIECES][32];
+__global__ void __launch_bounds__(256, 4) attn_extend_merge_kernel(const AxArgs p, int grid) {
+  __shared__ float s_m[AX_MAX_PIECES][32];
   pdl_wait();
   pdl_launch();
   const int32_t* d = p.desc + blockIdx.x * 8;
@@ -1123,22 +1123,26 @@ __global__ void __launch_bounds__(256) attn_extend_merge_kernel(const AxArgs p, 
   const int first = 2 * (static_cast<int>(blockIdx.x) - 1) + 1;        // then 2 * blockIdx.x, 2 * (blockIdx.x + 1), ...
   auto slot = [&](int i) -> size_t { return i == 0 ? first : 2 * (blockIdx.x + i - 1); };
   const float* ml = p.part + static_cast<size_t>(2 * grid) * p.rows * D;
-  for (int i = warp * subs + sub; i < pieces; i += 8 * subs) {
-    s_m[i][r] = live ? ml[slot(i) * 2 * p.rows + row] : -INFINITY;
-    s_l[i][r] = live ? ml[slot(i) * 2 * p.rows + p.rows + row] : 0.f;
+  constexpr int V = 4;           // float4s of a warp's columns
+  const int hd = head * p.grp + row % p.grp, col = blockIdx.z * 128 + warp * V * 4;
+  uint2 gv[V];
+  if (p.gate && live && sub == 0) {   // requested ahead of the partials
+    const uint2* g = reinterpret_cast<const uint2*>(p.gate + tok * p.gate_stride + static_cast<long long>(hd) * D + col);
+#pragma unroll
+    for (int c = 0; c < V; ++c) gv[c] = g[c];
   }
+  for (int i = warp * subs + sub; i < pieces; i += 8 * subs) s_m[i][r] = live ? ml[slot(i) * 2 * p.rows + row] : -INFINITY;
   __syncthreads();
   float M = -INFINITY;
   for (int i = sub; i < pieces; i += subs) M = fmaxf(M, s_m[i][r]);
   for (int o = span; o < 32; o <<= 1) M = fmaxf(M, __shfl_xor_sync(FULL_MASK, M, o));
-  constexpr int V = D / 32;      // float4s of a warp's columns
   float4 acc[V] = {};
   float L = 0.f;
-  const float4* part = reinterpret_cast<const float4*>(p.part) + static_cast<size_t>(warp * V) * p.rows + row;
+  const float4* part = reinterpret_cast<const float4*>(p.part) + static_cast<size_t>(col / 4) * p.rows + row;
 #pragma unroll 2
   for (int i = sub; i < pieces; i += subs) {
     const float m = s_m[i][r], w = m == -INFINITY ? 0.f : ax_exp2(m - M);
-    L = fmaf(s_l[i][r], w, L);
+    L = fmaf(live ? ml[slot(i) * 2 * p.rows + p.rows + row] : 0.f, w, L);
     const float4* x = part + slot(i) * (D / 4) * p.rows;
     float4 v[V];
 #pragma unroll
@@ -1163,18 +1167,15 @@ __global__ void __launch_bounds__(256) attn_extend_merge_kernel(const AxArgs p, 
   }
   if (!live || sub != 0) return;
   const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
-  const int hd = head * p.grp + row % p.grp, col = warp * V * 4;
-  const uint2* g = p.gate ? reinterpret_cast<const uint2*>(p.gate + tok * p.gate_stride + static_cast<long long>(hd) * D + col) : nullptr;
   uint2* o = reinterpret_cast<uint2*>(p.out + (static_cast<long long>(tok) * p.hq + hd) * D + col);
 #pragma unroll
   for (int c = 0; c < V; ++c) {
     float f[4] = {acc[c].x * inv, acc[c].y * inv, acc[c].z * inv, acc[c].w * inv};
-    if (g) {
-      const uint2 gv = g[c];
-      f[0] = __fdividef(f[0], 1.f + __expf(-bf_lo(gv.x)));
-      f[1] = __fdividef(f[1], 1.f + __expf(-bf_hi(gv.x)));
-      f[2] = __fdividef(f[2], 1.f + __expf(-bf_lo(gv.y)));
-      f[3] = __fdividef(f[3], 1.f + __expf(-bf_hi(gv.y)));
+    if (p.gate) {
+      f[0] = __fdividef(f[0], 1.f + __expf(-bf_lo(gv[c].x)));
+      f[1] = __fdividef(f[1], 1.f + __expf(-bf_hi(gv[c].x)));
+      f[2] = __fdividef(f[2], 1.f + __expf(-bf_lo(gv[c].y)));
+      f[3] = __fdividef(f[3], 1.f + __expf(-bf_hi(gv[c].y)));
     }
     o[c] = make_uint2(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]));
   }
@@ -1189,7 +1190,7 @@ static void ax_launch(const CUtensorMap& tmQ, const CUtensorMap& tmQs, const CUt
   once.run([] { cudaFuncSetAttribute(attn_extend_kernel<F8, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, X::SMEM); });
   const int grid = ax_grid();
   launch_k(attn_extend_kernel<F8, D>, dim3(grid), dim3(AX_THREADS), X::SMEM, st, tmQ, tmQs, tmK, tmV, a);
-  launch_k(attn_extend_merge_kernel<D>, dim3(grid, (a.rows + 31) / 32), dim3(256), 0, st, a, grid);
+  launch_k(attn_extend_merge_kernel<D>, dim3(grid, (a.rows + 31) / 32, D / 128), dim3(256), 0, st, a, grid);
 }
 
 // rows of a tile: the group's heads of as many tokens as fit 128 rows, or of all T
