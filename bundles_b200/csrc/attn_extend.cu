@@ -29,7 +29,7 @@
 // TMEM, so the scores of page t + NS wait for P . V of page t, and half of (softmax of a page, about 2600 cycles, + P . V,
 // scores and hand-overs, about 1700) is what a page takes with two buffers.  The exponential unit is busy 1024 of those.
 // Four 2048-token chunks behind 6144 tokens: 0.60 ms at first and 0.70 ms sustained (1545 MHz under the power limit),
-// 1.4 PFLOP/s.  Decode: 64 requests x 8192 tokens, 0.54 GB of e4m3 pages: 100 us, 114 us sustained (1440 MHz) = 4.7 TB/s.
+// 1.4 PFLOP/s.  Decode: 64 requests x 8192 tokens, 0.54 GB of e4m3 pages: 100 us, 107 us sustained (1440 MHz) = 5.0 TB/s.
 // Tried and dropped: four softmax warps per scheduler, each with half of a page (607 -> 650 us: more instructions, no
 // shorter chain); a quarter of the exponentials as a cubic on the FMA pipe (605 -> 610 us); polling instead of suspended
 // waits (650 -> 687 us: the pollers take the issue slots); 8 x 8 exchanges between lanes for an epilogue that writes whole

@@ -8,6 +8,7 @@ raise RuntimeError (qk_route.cu:1128-1133).
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from dataclasses import dataclass
 from typing import NamedTuple
 
@@ -569,9 +570,13 @@ def attn_extend(q, gate, kcache, vcache, page_table, cu_seqlens, seqlens, scale=
     return out
 
 
+@functools.lru_cache(maxsize=1024)
+def _attn_extend_bytes(T, heads, kv_heads, dim):
+    return max(_lib.lib().b200_attn_extend_workspace_bytes(T, heads, kv_heads, dim), 16)
+
+
 def attn_extend_workspace(T, heads, kv_heads, dim, device):
-    n = _lib.lib().b200_attn_extend_workspace_bytes(T, heads, kv_heads, dim)
-    return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
+    return torch.empty(_attn_extend_bytes(T, heads, kv_heads, dim), dtype=torch.uint8, device=device)
 
 
 def dense_fp8_workspace(T, H, device):

@@ -338,3 +338,26 @@ def test_values_that_are_not_finite_reach_the_rows_that_see_them_only(heads, dty
     assert fine.mean() > 0.5 and not fine.all()
     err = np.abs(got[fine] - ref[fine])
     assert (err <= 2.0 ** -8 * np.abs(ref[fine]) + 2.125 * 2.0 ** -8 * spread[fine]).all()
+
+
+@pytest.mark.parametrize("dtype", ["e4m3", "bf16"])
+def test_abandoned_waits_wind_down(dtype):
+    """With a wait budget of one nanosecond the first wait that is not over at once gives up: the call ends with a status code,
+    every role returns, and the next ordinary call gives the same bits as before."""
+    from bundles_b200 import ops
+    d, scale = pu.make([(300, 2000), (1, 5000), (70, 64)], dtype, seed=95)
+    c = pu.on(d, DEV)
+    want = ops.attn_extend(**c, scale=scale)
+    torch.cuda.synchronize()
+    bad = ops.new_status(DEV)
+    ops.set_wait_budget_ns(1)
+    try:
+        ops.attn_extend(**c, scale=scale, status=bad)
+        torch.cuda.synchronize()
+    finally:
+        ops.set_wait_budget_ns(0)
+    assert ops.read_status(bad) in range(101, 107)
+    st = ops.new_status(DEV)
+    again = ops.attn_extend(**c, scale=scale, status=st)
+    torch.cuda.synchronize()
+    assert ops.read_status(st) == 0 and torch.equal(again, want)
