@@ -54,8 +54,6 @@ constexpr int AX_THREADS = AX_WARPS * 32;
 constexpr int AX_SOFT0 = 4, AX_SOFT = 8;
 
 struct AxArgs {
-  const void* q;
-  long long q_stride;
   const bf16* gate;
   long long gate_stride;
   const void* vc;
@@ -1253,8 +1251,6 @@ extern "C" int b200_attn_extend(const void* q, long long q_stride, const void* g
                                AX_PAGE, "k cache")))
     return rc;
   if ((rc = make_tmap_bytes_2d(&tmV, vcache, static_cast<uint64_t>(num_pages) * Hkv * D, AX_PAGE * es, D, "v cache"))) return rc;
-  a.q = q;
-  a.q_stride = q_stride;
   a.gate = static_cast<const bf16*>(gate);
   a.gate_stride = gate_stride;
   a.vc = vcache;
